@@ -12,11 +12,15 @@ Reference API mirrored here:
     require_cuda_contiguous, SUPPORTED_M/K/N/EXTRA_SHAPES
 Added for the decode paths this package also covers:
     w4a16_linear_f32, w4a16_gate_up_silu, decode_mlp, gqa_decode_attention,
-    baseline_case, check_shape
+    baseline_case, check_shape,
+    rope, rope_inv_freq, kv8_cache, kv8_append, gqa_decode_attention_kv8,
+    decode_attention_kv8
 """
 from __future__ import annotations
 
+import math
 from importlib import import_module
+from typing import NamedTuple
 
 import torch
 
@@ -213,20 +217,171 @@ def gqa_decode_attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: 
     return _ext().gqa_decode_attention_paged(q, k_pages, v_pages, block_table, seq_lens, max_seq_len, scale)
 
 
+# ---------------------------------------- rotary positions, 8-bit KV cache
+def rope_inv_freq(rot: int, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
+                  original_max_position: int = 4096, low: float = 1.0, high: float = 32.0,
+                  device="cuda") -> tuple[torch.Tensor, float]:
+    """(inv_freq, mscale) for `rope` and `kv8_append`: fp64 [rot / 2] radians
+    per position, base^(-2i / rot), and the factor on cos and sin.
+
+    scaling, for contexts `factor` times the trained `original_max_position`:
+      None      as trained
+      "linear"  inv_freq / factor
+      "ntk"     base * factor^(rot / (rot - 2)) in place of base
+      "yarn"    pairs that turn less than `low` times over the original length
+                are divided by factor, those that turn more than `high` times
+                are kept, with a linear ramp over the pairs between (rounded
+                outwards to whole pairs); mscale is 0.1 ln(factor) + 1
+      "bands"   as "yarn" with the ramp in the number of turns itself, from `low`
+                to `high`; mscale is 1
+    """
+    if rot < 2 or rot % 2 != 0:
+        raise ValueError("rot must be even and positive")
+    if not base > 1.0 or not factor >= 1.0:
+        raise ValueError("base must be above 1 and factor at least 1")
+    f = [base ** (-2.0 * i / rot) for i in range(rot // 2)]
+    mscale = 1.0
+    if scaling == "linear":
+        f = [x / factor for x in f]
+    elif scaling == "ntk":
+        if rot < 4:
+            raise ValueError("ntk scaling needs rot >= 4")
+        wide = base * factor ** (rot / (rot - 2.0))
+        f = [wide ** (-2.0 * i / rot) for i in range(rot // 2)]
+    elif scaling in ("yarn", "bands"):
+        if not 0.0 < low < high or original_max_position < 1:
+            raise ValueError("low must be positive and below high, original_max_position positive")
+        if scaling == "yarn":
+            def pair(turns):  # the fractional pair that turns so often over the original length
+                return rot * math.log(original_max_position / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+            first, last = max(math.floor(pair(high)), 0), min(math.ceil(pair(low)), rot // 2 - 1)
+            keep = [1.0 - min(1.0, max(0.0, (i - first) / max(last - first, 0.001))) for i in range(rot // 2)]
+            mscale = 0.1 * math.log(factor) + 1.0
+        else:
+            turns = [original_max_position * x / (2 * math.pi) for x in f]
+            keep = [min(1.0, max(0.0, (t - low) / (high - low))) for t in turns]
+        f = [x * k + x / factor * (1.0 - k) for x, k in zip(f, keep)]
+    elif scaling is not None:
+        raise ValueError(f"unknown scaling: {scaling}")
+    return torch.tensor(f, dtype=torch.float64, device=device), mscale
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool = False,
+         mscale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions: the first 2 * len(inv_freq) dims of x [T, H, D] turned by
+    positions[t] * inv_freq[i]; pairs are dims (i, i + rot / 2), or (2i, 2i + 1)
+    with `interleaved`.
+
+    x is bf16, fp16 or fp32 with a contiguous last dimension (a view of packed
+    QKV rows will do); positions int32 or int64 [T]; inv_freq fp64.  Angles, cos
+    and sin are 64-bit, the turn fp32, with one rounding.  Writes a new
+    contiguous tensor, or `out` (x itself works in place).
+    """
+    return _ext().rope(x, positions, inv_freq, interleaved, mscale, out)
+
+
+class Kv8Cache(NamedTuple):
+    """An 8-bit paged KV cache: codes [num_pages, Hkv, page_size, D] and fp32
+    scales [num_pages, Hkv, page_size / 16]; a code c stands for c * scale."""
+
+    k_pages: torch.Tensor
+    v_pages: torch.Tensor
+    k_scales: torch.Tensor
+    v_scales: torch.Tensor
+
+
+def kv8_cache(num_pages: int, Hkv: int, page_size: int, D: int = 128, dtype: torch.dtype = torch.float8_e4m3fn,
+              device="cuda") -> Kv8Cache:
+    """An empty 8-bit paged KV cache (dtype float8_e4m3fn or int8)."""
+    if dtype not in (torch.float8_e4m3fn, torch.int8):
+        raise ValueError("dtype must be torch.float8_e4m3fn or torch.int8")
+    if page_size not in (16, 32) and (page_size < 64 or page_size % 64 != 0):
+        raise ValueError("page_size must be 16, 32 or a multiple of 64")
+    if D not in (64, 128):
+        raise ValueError("D must be 64 or 128")
+    pages = [torch.zeros((num_pages, Hkv, page_size, D), dtype=torch.uint8, device=device).view(dtype) for _ in "kv"]
+    scales = [torch.zeros((num_pages, Hkv, page_size // 16), dtype=torch.float32, device=device) for _ in "kv"]
+    return Kv8Cache(*pages, *scales)
+
+
+def kv8_append(k: torch.Tensor, v: torch.Tensor, cache, block_table: torch.Tensor, seq_lens: torch.Tensor,
+               cu_new: torch.Tensor | None = None, max_new: int | None = None, q: torch.Tensor | None = None,
+               inv_freq: torch.Tensor | None = None, interleaved: bool = False,
+               mscale: float = 1.0) -> torch.Tensor | None:
+    """Append new tokens' keys and values to an 8-bit paged cache, in place.
+
+    k, v [T, Hkv, D] bf16 or fp16 (strided rows will do); sequence b's new
+    tokens are rows cu_new[b] .. cu_new[b + 1] - 1 (int32 [B + 1] on the device,
+    none of them more than max_new, a host integer), or without cu_new T / B rows
+    each.  They become the last positions of seq_lens[b] (int32 [B]), which counts
+    them already; block_table int32 [B, max_pages].  With inv_freq, k is turned by
+    its positions first (see rope) and so is q [T, Hq, D], which is returned.
+
+    Every 16 consecutive tokens of a page and head share a scale: e4m3 the
+    smallest power of two >= amax / 448, int8 amax / 127.  It grows when later
+    tokens of the block need it; the earlier ones' codes are then moved to it.
+    A page that receives tokens must belong to one sequence of the call.
+    """
+    if max_new is None:
+        if cu_new is not None:
+            raise ValueError("cu_new needs max_new")
+        B = seq_lens.shape[0]
+        if B == 0 or k.shape[0] % B != 0:
+            raise ValueError("without cu_new, every sequence must have the same number of new tokens")
+        max_new = k.shape[0] // B
+    return _ext().kv8_append(k, v, *cache, block_table, seq_lens, cu_new, max_new, q, inv_freq, interleaved, mscale)
+
+
+def gqa_decode_attention_kv8(q: torch.Tensor, cache, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                             max_seq_len: int, scale: float | None = None) -> torch.Tensor:
+    """Decode attention over an 8-bit paged KV cache with per-sequence lengths.
+
+    q [B, Hq, D], or [B, T, Hq, D] for the last T <= 16 positions of each sequence
+    (query t sees positions < seq_lens[b] - T + 1 + t), bf16 or fp16; cache as
+    kv8_append writes it; block_table int32 [B, max_pages]; seq_lens int32 [B] in
+    0..max_seq_len (a host integer that sizes the launch).  A query that sees no
+    position gives zeros.  D is 64 or 128; scale defaults to 1/sqrt(D).
+    """
+    return _ext().gqa_decode_attention_kv8(q, *cache, block_table, seq_lens, max_seq_len, scale)
+
+
+def decode_attention_kv8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache, block_table: torch.Tensor,
+                         seq_lens: torch.Tensor, max_seq_len: int, inv_freq: torch.Tensor,
+                         interleaved: bool = False, mscale: float = 1.0, scale: float | None = None) -> torch.Tensor:
+    """The attention of a decode step behind its QKV projection: q [B * T, Hq, D],
+    k and v [B * T, Hkv, D] (T new tokens per sequence, counted by seq_lens
+    already) are turned, k and v appended, and the queries attend over the cache.
+    Returns o [B * T, Hq, D]."""
+    turned = kv8_append(k, v, cache, block_table, seq_lens, q=q, inv_freq=inv_freq, interleaved=interleaved,
+                        mscale=mscale)
+    B = seq_lens.shape[0]
+    o = gqa_decode_attention_kv8(turned.view(B, -1, *turned.shape[1:]), cache, block_table, seq_lens, max_seq_len,
+                                 scale)
+    return o.view(turned.shape)
+
+
 __all__ = [
+    "Kv8Cache",
     "SUPPORTED_K",
     "SUPPORTED_M",
     "SUPPORTED_N",
     "SUPPORTED_EXTRA_SHAPES",
     "baseline_case",
     "check_shape",
+    "decode_attention_kv8",
     "decode_mlp",
     "dequant_ref",
     "gqa_decode_attention",
+    "gqa_decode_attention_kv8",
     "gqa_decode_attention_paged",
+    "kv8_append",
+    "kv8_cache",
     "pack_int4_weight",
     "random_case",
     "require_cuda_contiguous",
+    "rope",
+    "rope_inv_freq",
     "w4a16_gate_up_silu",
     "w4a16_linear",
     "w4a16_linear_f32",

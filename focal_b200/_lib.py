@@ -22,6 +22,11 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _S = ctypes.c_size_t
 _F = ctypes.c_float
+_L = ctypes.c_int64
+
+# enum focal_dtype and enum focal_code
+FOCAL_BF16, FOCAL_FP16, FOCAL_FP32 = 0, 1, 2
+FOCAL_E4M3, FOCAL_INT8 = 0, 1
 
 
 class TpComm(ctypes.Structure):
@@ -31,7 +36,25 @@ class TpComm(ctypes.Structure):
                 ("world", ctypes.c_int), ("rank", ctypes.c_int)]
 
 
+class Kv8Cache(ctypes.Structure):
+    """struct focal_kv8_cache: the pages and scales of an 8-bit KV cache."""
+
+    _fields_ = [("k_pages", _P), ("v_pages", _P), ("k_scales", _P), ("v_scales", _P), ("num_pages", _I),
+                ("num_kv_heads", _I), ("page_size", _I), ("head_dim", _I), ("code", _I)]
+
+
+class Kv8AppendArgs(ctypes.Structure):
+    """struct focal_kv8_append_args."""
+
+    _fields_ = [("k", _P), ("v", _P), ("q", _P), ("q_out", _P), ("block_table", _P), ("seq_lens", _P),
+                ("cu_new", _P), ("inv_freq", _P), ("k_token_stride", _L), ("k_head_stride", _L),
+                ("v_token_stride", _L), ("v_head_stride", _L), ("q_token_stride", _L), ("q_head_stride", _L),
+                ("B", _I), ("T", _I), ("max_new", _I), ("Hq", _I), ("max_pages_per_seq", _I), ("rot", _I),
+                ("interleaved", _I), ("dtype", _I), ("mscale", ctypes.c_double)]
+
+
 _C = ctypes.POINTER(TpComm)
+_K = ctypes.POINTER(Kv8Cache)
 
 # name -> (restype, argtypes); mirrors include/focal_b200.h
 SIGNATURES = {
@@ -62,6 +85,11 @@ SIGNATURES = {
     "focal_gqa_decode_workspace_size": (_S, [_I, _I, _I, _I, _I]),
     "focal_gqa_decode_attn": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _S, _P]),
     "focal_gqa_decode_paged": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _S, _P]),
+    "focal_rope": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, ctypes.c_double, _I, _I, _L, _L, _L, _L, _P]),
+    "focal_kv8_append": (_I, [ctypes.POINTER(Kv8AppendArgs), _K, _P]),
+    "focal_kv8_decode_workspace_size": (_S, [_I, _I, _I, _I, _I, _I]),
+    "focal_kv8_decode_counter_bytes": (_S, [_I, _I, _I, _I]),
+    "focal_kv8_decode": (_I, [_P, _P, _K, _P, _P, _I, _I, _I, _I, _I, _F, _I, _P, _S, _P]),
     "focal_device_status": (_I, [ctypes.POINTER(_I)]),
     "focal_device_status_peek": (_I, [ctypes.POINTER(_I)]),
     "focal_reset_device_status": (_I, []),

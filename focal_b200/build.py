@@ -33,8 +33,9 @@ INCLUDE = ROOT / "include"
 BUILD = ROOT / "_build"
 LIB = PKG / "libfocal_b200.so"
 TIMELINE_LIB = PKG / "libfocal_b200_timeline.so"
-CU_SOURCES = ["capi.cu", "w4a16_gemv.cu", "w4a16_tiles.cu", "gqa_decode.cu"]
-HEADERS = ["common.cuh", "host_common.h", "w4a16_tiles.h"]
+CU_SOURCES = ["capi.cu", "w4a16_gemv.cu", "w4a16_tiles.cu", "gqa_decode.cu", "rope.cu", "kv8_append.cu",
+              "kv8_decode.cu"]
+HEADERS = ["common.cuh", "host_common.h", "w4a16_tiles.h", "kv8_common.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1,0 +1,339 @@
+// Append to the 8-bit paged KV cache: a step's or a prompt's keys and values,
+// quantised to e4m3 or int8 codes with one fp32 scale per block of 16
+// consecutive tokens and KV head, written into the sequences' pages.  Keys (and
+// the queries, which are returned) can be turned by their rotary positions on
+// the way, so a decode step needs one launch between its QKV projection and its
+// attention.
+//
+// For the rows of a block that a call brings, amax = max |x|, and
+//   e4m3: need = the smallest power of two >= amax / 448
+//   int8: need = amax / 127
+//   scale = max(old scale, need); the old scale counts as 0 when the block's
+//   first row is among the new ones
+//   code  = round-to-nearest-even(x / scale)
+// When the scale of a block that holds older rows grows, those rows' codes are
+// moved to it.  With powers of two that is exact for e4m3 but for codes that
+// sink below its smallest subnormal; e4m3 loses nothing by it, since a
+// floating-point code's relative precision does not depend on the scale.  int8
+// does lose precision with a scale larger than needed, so it takes amax / 127 and pays
+// one more rounding when a block grows.
+//
+// One warp takes one (block, head) of K or of V, or 16 rows of one query head:
+// a lane holds 8 dims of every (32 / (D / 8))-th row in fp32 registers, so the
+// rows are read once and amax needs one warp reduction.  The cos and sin of the
+// block's rows are computed once per thread block into shared memory.
+#include <algorithm>
+#include <cmath>
+
+#include "kv8_common.cuh"
+
+namespace focal {
+namespace kv8 {
+
+constexpr int kAppendWarps = 8;
+constexpr float kMinScale = 1.17549435e-38f;  // 2^-126: scales stay normal numbers
+
+struct AppendParams {
+  const void *k, *v, *q;
+  void* q_out;
+  uint8_t *k_pages, *v_pages;
+  float *k_scales, *v_scales;
+  const int32_t *block_table, *seq_lens, *cu_new;
+  const double* inv_freq;
+  int* status;
+  long long kt, kh, vt, vh, qt, qh;  // strides in elements
+  int T, max_new, Hq, Hkv, half, num_pages, page_size, max_pages, pieces, jobs_per_block;
+  double mscale;
+};
+
+// The scale that amax needs (0 for amax = 0: codes 0, and any later scale is larger).
+template <bool INT8>
+__device__ __forceinline__ float needed_scale(float amax) {
+  if (amax == 0.f) return 0.f;
+  if (INT8) return fmaxf(__fdiv_rn(amax, 127.f), kMinScale);
+  const float r = fmaxf(__fdiv_rn(amax, 448.f), kMinScale);
+  const uint32_t up = (__float_as_uint(r) + 0x7FFFFFu) & 0x7F800000u;  // next power of two
+  return __uint_as_float(up);
+}
+
+__device__ __forceinline__ uint32_t int8_code(float r) {
+  const int c = __float2int_rn(r);  // NaN gives 0
+  return static_cast<uint32_t>(max(-127, min(127, c))) & 0xFFu;
+}
+
+// Four codes of x / scale; scale > 0.
+template <bool INT8>
+__device__ __forceinline__ uint32_t quantise4(const float* x, float scale) {
+  if (INT8)
+    return int8_code(__fdiv_rn(x[0], scale)) | int8_code(__fdiv_rn(x[1], scale)) << 8 |
+           int8_code(__fdiv_rn(x[2], scale)) << 16 | int8_code(__fdiv_rn(x[3], scale)) << 24;
+  return f32x2_to_e4m3x2(__fdiv_rn(x[0], scale), __fdiv_rn(x[1], scale)) |
+         static_cast<uint32_t>(f32x2_to_e4m3x2(__fdiv_rn(x[2], scale), __fdiv_rn(x[3], scale))) << 16;
+}
+
+template <bool INT8>
+__device__ __forceinline__ void dequantise4(uint32_t c, float (&x)[4]) {
+  if (INT8) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = static_cast<float>(static_cast<int8_t>(c >> (8 * e)));
+  } else {
+    const uint32_t lo = e4m3x2_to_f16x2(c & 0xFFFFu), hi = e4m3x2_to_f16x2(c >> 16);
+    x[0] = half_lo(lo);
+    x[1] = half_hi(lo);
+    x[2] = half_lo(hi);
+    x[3] = half_hi(hi);
+  }
+}
+
+template <typename T, int D, bool INT8, bool INTERLEAVED>
+__global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(const AppendParams p) {
+  constexpr int kLanes = D / 8;           // lanes of one row
+  constexpr int kRows = 32 / kLanes;      // rows that a warp holds side by side
+  constexpr int kPasses = kGroup / kRows;
+  __shared__ float2 cs[kGroup][D / 2];
+  griddep_launch_dependents();
+  griddep_wait();
+
+  const int b = blockIdx.x / p.pieces;
+  const int len = p.seq_lens[b];
+  const int c0 = p.cu_new ? p.cu_new[b] : b * p.max_new;
+  const int c1 = p.cu_new ? p.cu_new[b + 1] : c0 + p.max_new;
+  const int n = c1 - c0;
+  if (c0 < 0 || c1 > p.T || c1 < c0 || n > p.max_new || len < n || len > (long long)p.max_pages * p.page_size) {
+    if (threadIdx.x == 0) set_status(p.status, kDevBadIndex);
+    return;
+  }
+  const int start = len - n;  // position of the first new row
+  const long long at0 = ((long long)(start / kGroup) + blockIdx.x % p.pieces) * kGroup;
+  if (n == 0 || at0 >= len) return;
+  const int at = static_cast<int>(at0);  // position of the block's row 0
+  const int r0 = max(start - at, 0), r1 = min(len - at, kGroup);  // the new rows of the block
+  const int page = p.block_table[(long long)b * p.max_pages + at / p.page_size];
+  if (page < 0 || page >= p.num_pages) {
+    if (threadIdx.x == 0) set_status(p.status, kDevBadIndex);
+    return;
+  }
+  const int tok = c0 + at - start;  // token of row r: tok + r
+  for (int i = threadIdx.x; i < (r1 - r0) * p.half; i += 32 * kAppendWarps) {
+    const int r = i / p.half, f = i - r * p.half;
+    cs[r0 + r][f] = rope_cos_sin(static_cast<double>(at + r0 + r), p.inv_freq[f], p.mscale);
+  }
+  __syncthreads();
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c = lane % kLanes, rr = lane / kLanes;
+  const int rot = 2 * p.half;
+  // this lane's dims: d0 .. d0 + 3 and d1 .. d1 + 3; with `turns`, four pairs of frequencies 4c .. 4c + 3
+  const bool turns = INTERLEAVED ? 8 * c < rot : 4 * c < p.half;
+  int d0, d1;
+  if (INTERLEAVED) {
+    d0 = 8 * c;
+    d1 = d0 + 4;
+  } else {
+    d0 = turns ? 4 * c : 8 * c;
+    d1 = turns ? p.half + 4 * c : d0 + 4;
+  }
+  const int sub = at % p.page_size;  // row of the page
+  const int jobs = 2 * p.Hkv + p.Hq;
+  const int j1 = min(jobs, static_cast<int>(blockIdx.y + 1) * p.jobs_per_block);
+  for (int j = blockIdx.y * p.jobs_per_block + warp; j < j1; j += kAppendWarps) {
+    const bool is_q = j >= 2 * p.Hkv, is_v = !is_q && j >= p.Hkv;
+    const int h = is_q ? j - 2 * p.Hkv : is_v ? j - p.Hkv : j;
+    const long long ts = is_q ? p.qt : is_v ? p.vt : p.kt, hs = is_q ? p.qh : is_v ? p.vh : p.kh;
+    const T* x = static_cast<const T*>(is_q ? p.q : is_v ? p.v : p.k) + h * hs;
+    float val[kPasses][8];
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = i * kRows + rr;
+      uint2 u = make_uint2(0u, 0u), w = make_uint2(0u, 0u);
+      if (r >= r0 && r < r1) {
+        const T* row = x + (long long)(tok + r) * ts;
+        u = *reinterpret_cast<const uint2*>(row + d0);
+        w = *reinterpret_cast<const uint2*>(row + d1);
+      }
+      const float2 f0 = unpack2<T>(u.x), f1 = unpack2<T>(u.y), f2 = unpack2<T>(w.x), f3 = unpack2<T>(w.y);
+      val[i][0] = f0.x; val[i][1] = f0.y; val[i][2] = f1.x; val[i][3] = f1.y;
+      val[i][4] = f2.x; val[i][5] = f2.y; val[i][6] = f3.x; val[i][7] = f3.y;
+    }
+    if (!is_v && turns) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = i * kRows + rr;
+        if (r >= r0 && r < r1) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            rope_turn(INTERLEAVED ? val[i][2 * e] : val[i][e], INTERLEAVED ? val[i][2 * e + 1] : val[i][4 + e],
+                      cs[r][4 * c + e]);
+        }
+      }
+    }
+    if (is_q) {
+      T* y = static_cast<T*>(p.q_out) + (long long)h * D;
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = i * kRows + rr;
+        if (r >= r0 && r < r1) {
+          T* row = y + (long long)(tok + r) * p.Hq * D;
+          *reinterpret_cast<uint2*>(row + d0) = make_uint2(pack2<T>(val[i][0], val[i][1]), pack2<T>(val[i][2], val[i][3]));
+          *reinterpret_cast<uint2*>(row + d1) = make_uint2(pack2<T>(val[i][4], val[i][5]), pack2<T>(val[i][6], val[i][7]));
+        }
+      }
+      continue;
+    }
+    // infinities saturate and NaN is stored as NaN (e4m3) or 0 (int8); neither sets the scale
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float m = fabsf(val[i][e]);
+        if (m < INFINITY) amax = fmaxf(amax, m);
+      }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    uint8_t* pages = is_v ? p.v_pages : p.k_pages;
+    float* scales = is_v ? p.v_scales : p.k_scales;
+    const long long ph = (long long)page * p.Hkv + h;
+    uint8_t* out = pages + (ph * p.page_size + sub) * D;
+    float* sp = scales + ph * (p.page_size / kGroup) + sub / kGroup;
+    const float old = r0 > 0 ? *sp : 0.f;
+    const float scale = fmaxf(old, needed_scale<INT8>(amax));
+    if (r0 > 0 && scale > old) {
+      for (int r = rr; r < r0; r += kRows) {
+        uint32_t* a0 = reinterpret_cast<uint32_t*>(out + r * D + d0);
+        uint32_t* a1 = reinterpret_cast<uint32_t*>(out + r * D + d1);
+        float f[4], g[4];
+        dequantise4<INT8>(*a0, f);
+        dequantise4<INT8>(*a1, g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f[e] *= old;
+          g[e] *= old;
+        }
+        *a0 = quantise4<INT8>(f, scale);
+        *a1 = quantise4<INT8>(g, scale);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = i * kRows + rr;
+      if (r >= r0 && r < r1) {
+        *reinterpret_cast<uint32_t*>(out + r * D + d0) = scale > 0.f ? quantise4<INT8>(val[i], scale) : 0u;
+        *reinterpret_cast<uint32_t*>(out + r * D + d1) = scale > 0.f ? quantise4<INT8>(val[i] + 4, scale) : 0u;
+      }
+    }
+    __syncwarp();
+    if (lane == 0) *sp = scale;
+  }
+}
+
+int check_cache(const focal_kv8_cache* c) {
+  if (!c) return set_error(FOCAL_ERR_INVALID_VALUE, "null cache");
+  if (c->code != FOCAL_E4M3 && c->code != FOCAL_INT8)
+    return set_error(FOCAL_ERR_UNSUPPORTED, "unsupported cache code (must be e4m3 or int8)");
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return set_error(FOCAL_ERR_UNSUPPORTED, "unsupported head_dim (must be 64 or 128)");
+  if (c->num_pages < 1 || c->num_kv_heads < 1)
+    return set_error(FOCAL_ERR_UNSUPPORTED, "num_pages and num_kv_heads must be positive");
+  if (c->page_size != 16 && c->page_size != 32 && (c->page_size < 64 || c->page_size % 64 != 0))
+    return set_error(FOCAL_ERR_UNSUPPORTED, "page_size must be 16, 32 or a multiple of 64");
+  return FOCAL_OK;
+}
+
+int check_cache_pointers(const focal_kv8_cache* c) {
+  if (!c->k_pages || !c->v_pages || !c->k_scales || !c->v_scales)
+    return set_error(FOCAL_ERR_INVALID_VALUE, "null pointer");
+  if (!aligned(c->k_pages, 16) || !aligned(c->v_pages, 16) || !aligned(c->k_scales, 16) || !aligned(c->v_scales, 16))
+    return set_error(FOCAL_ERR_INVALID_VALUE, "pages and scales must be 16-byte aligned");
+  return FOCAL_OK;
+}
+
+template <typename T, int D>
+int launch_append(const AppendParams& p, int code, bool interleaved, dim3 grid, cudaStream_t s) {
+  const char* what = "append_kernel launch";
+  const int n = 32 * kAppendWarps;
+  if (code == FOCAL_INT8)
+    return interleaved ? launch_pdl(append_kernel<T, D, true, true>, grid, n, 0, s, what, p)
+                       : launch_pdl(append_kernel<T, D, true, false>, grid, n, 0, s, what, p);
+  return interleaved ? launch_pdl(append_kernel<T, D, false, true>, grid, n, 0, s, what, p)
+                     : launch_pdl(append_kernel<T, D, false, false>, grid, n, 0, s, what, p);
+}
+
+}  // namespace kv8
+}  // namespace focal
+
+using namespace focal;
+
+extern "C" int focal_kv8_append(const focal_kv8_append_args* a, const focal_kv8_cache* cache, cudaStream_t stream) {
+  using namespace kv8;
+  clear_error();
+  if (!a) return set_error(FOCAL_ERR_INVALID_VALUE, "null arguments");
+  int rc = check_cache(cache);
+  if (rc) return rc;
+  const int D = cache->head_dim, Hkv = cache->num_kv_heads;
+  if (a->dtype != FOCAL_BF16 && a->dtype != FOCAL_FP16)
+    return set_error(FOCAL_ERR_UNSUPPORTED, "unsupported dtype (must be bf16 or fp16)");
+  if (a->B < 0 || a->T < 0 || a->max_new < 0 || a->Hq < 0 || a->max_pages_per_seq < 1)
+    return set_error(FOCAL_ERR_UNSUPPORTED, "B, T, max_new and Hq must not be negative, max_pages_per_seq positive");
+  if (!a->cu_new && (long long)a->B * a->max_new != a->T)
+    return set_error(FOCAL_ERR_UNSUPPORTED, "without cu_new, T must be B * max_new");
+  if (a->rot != 0 && (a->rot < 16 || a->rot % 16 != 0 || a->rot > D))
+    return set_error(FOCAL_ERR_UNSUPPORTED, "the rotated dims must be a multiple of 16, at most D");
+  if (a->Hq > 0 && a->rot == 0) return set_error(FOCAL_ERR_UNSUPPORTED, "q is only turned: it needs rotated dims");
+  if (!std::isfinite(a->mscale)) return set_error(FOCAL_ERR_INVALID_VALUE, "mscale must be finite");
+  if (a->k_token_stride % 8 || a->k_head_stride % 8 || a->v_token_stride % 8 || a->v_head_stride % 8 ||
+      a->q_token_stride % 8 || a->q_head_stride % 8)
+    return set_error(FOCAL_ERR_UNSUPPORTED, "token and head strides must be multiples of 16 bytes");
+  const long long pieces = ((long long)a->max_new + 30) / kGroup;  // blocks that max_new rows can touch
+  if (pieces * a->B > INT32_MAX) return set_error(FOCAL_ERR_UNSUPPORTED, "B * max_new too large");
+  if (a->B == 0 || a->T == 0 || a->max_new == 0) return FOCAL_OK;
+  rc = check_cache_pointers(cache);
+  if (rc) return rc;
+  if (!a->k || !a->v || !a->block_table || !a->seq_lens || (a->rot && !a->inv_freq) || (a->Hq && (!a->q || !a->q_out)))
+    return set_error(FOCAL_ERR_INVALID_VALUE, "null pointer");
+  if (!aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->q, 16) || !aligned(a->q_out, 16) ||
+      !aligned(a->block_table, 4) || !aligned(a->seq_lens, 4) || !aligned(a->cu_new, 4) || !aligned(a->inv_freq, 8))
+    return set_error(FOCAL_ERR_INVALID_VALUE, "k, v and q must be 16-byte, tables 4-byte, inv_freq 8-byte aligned");
+  DeviceInfo dev;
+  rc = current_device_info(&dev);
+  if (rc) return rc;
+  AppendParams p{};
+  p.k = a->k;
+  p.v = a->v;
+  p.q = a->q;
+  p.q_out = a->q_out;
+  p.k_pages = static_cast<uint8_t*>(cache->k_pages);
+  p.v_pages = static_cast<uint8_t*>(cache->v_pages);
+  p.k_scales = cache->k_scales;
+  p.v_scales = cache->v_scales;
+  p.block_table = a->block_table;
+  p.seq_lens = a->seq_lens;
+  p.cu_new = a->cu_new;
+  p.inv_freq = a->inv_freq;
+  p.status = dev.status;
+  p.kt = a->k_token_stride;
+  p.kh = a->k_head_stride;
+  p.vt = a->v_token_stride;
+  p.vh = a->v_head_stride;
+  p.qt = a->q_token_stride;
+  p.qh = a->q_head_stride;
+  p.T = a->T;
+  p.max_new = a->max_new;
+  p.Hq = a->Hq;
+  p.Hkv = Hkv;
+  p.half = a->rot / 2;
+  p.num_pages = cache->num_pages;
+  p.page_size = cache->page_size;
+  p.max_pages = a->max_pages_per_seq;
+  p.pieces = static_cast<int>(pieces);
+  p.mscale = a->mscale;
+  const int jobs = 2 * Hkv + a->Hq;
+  p.jobs_per_block = jobs;
+  const dim3 grid(static_cast<unsigned>(pieces * a->B), 1, 1);
+  const bool il = a->interleaved != 0;
+  if (a->dtype == FOCAL_BF16)
+    return D == 128 ? launch_append<__nv_bfloat16, 128>(p, cache->code, il, grid, stream)
+                    : launch_append<__nv_bfloat16, 64>(p, cache->code, il, grid, stream);
+  return D == 128 ? launch_append<__half, 128>(p, cache->code, il, grid, stream)
+                  : launch_append<__half, 64>(p, cache->code, il, grid, stream);
+}

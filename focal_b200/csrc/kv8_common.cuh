@@ -1,0 +1,93 @@
+// Shared by the rotary, 8-bit cache append and 8-bit cache attention kernels:
+// code conversions, the angle of a position, and the programmatic launch.
+#pragma once
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "host_common.h"
+
+namespace focal {
+namespace kv8 {
+
+constexpr int kGroup = 16;  // consecutive tokens of a page and KV head that share a scale
+
+// Two e4m3 codes (low byte first) as f16x2; every e4m3 value is exact in f16.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t c) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(c));
+  return r;
+}
+
+// Two floats as e4m3 codes (`lo` in the low byte), nearest even, saturating at
+// 448; NaN stays NaN.
+__device__ __forceinline__ uint16_t f32x2_to_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// cos and sin of position * inv_freq, times mscale, each rounded once to fp32.
+// The angle and its reduction are 64-bit: at position 2^20 an fp32 angle is
+// off by up to 2^-5 radians, a 64-bit one by 2^-34.
+__device__ __forceinline__ float2 rope_cos_sin(double position, double inv_freq, double mscale) {
+  double s, c;
+  sincos(__dmul_rn(position, inv_freq), &s, &c);
+  return make_float2(static_cast<float>(__dmul_rn(c, mscale)), static_cast<float>(__dmul_rn(s, mscale)));
+}
+
+// (a, b) turned by the angle of (cos, sin): products and sums each rounded to
+// fp32 (no contraction), so the result does not depend on how the compiler
+// would pair them.
+__device__ __forceinline__ void rope_turn(float& a, float& b, float2 cs) {
+  const float u = __fsub_rn(__fmul_rn(a, cs.x), __fmul_rn(b, cs.y));
+  b = __fadd_rn(__fmul_rn(a, cs.y), __fmul_rn(b, cs.x));
+  a = u;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T x) {
+  return static_cast<float>(x);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);  // one 32-bit word, one rounding each
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  return pack_bf16x2(lo, hi);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(bf16_lo(w), bf16_hi(w));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return make_float2(half_lo(w), half_hi(w));
+}
+
+// Launch with programmatic stream serialisation: the kernel's set-up may
+// overlap the previous kernel; it touches memory only after griddep_wait().
+template <typename... P, typename... A>
+int launch_pdl(void (*kern)(P...), dim3 grid, int threads, int smem, cudaStream_t stream, const char* what,
+               A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, args...), what);
+}
+
+}  // namespace kv8
+}  // namespace focal

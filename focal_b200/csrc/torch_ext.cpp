@@ -7,6 +7,7 @@
 // torch::empty on x's device; work is queued on PyTorch's current stream under
 // a device guard; failures raise RuntimeError with the reference's messages.
 // All arithmetic happens in libfocal_b200.so behind include/focal_b200.h.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -41,7 +42,7 @@ cudaStream_t current_stream() {
 // Their partial words start at zero and every successful call leaves them at zero,
 // and calls on one stream are ordered, so reuse is safe.  A workspace that is
 // outgrown stays allocated (a CUDA graph captured earlier may still use it).
-enum WsKind { kWsLinear = 0, kWsAttention = 1 };
+enum WsKind { kWsLinear = 0, kWsAttention = 1, kWsKv8 = 2 };
 std::mutex g_ws_mutex;
 std::map<std::tuple<int, int, cudaStream_t>, torch::Tensor> g_ws;
 std::vector<torch::Tensor> g_ws_retired;
@@ -83,6 +84,38 @@ torch::Tensor workspace_for(WsKind kind, const torch::Device& dev, cudaStream_t 
     return t;
   }
   return it->second;
+}
+
+// A workspace for a call that may be captured.  Outside a capture it is
+// workspace_for's.  Inside one it belongs to that capture and stream: allocated
+// from the graph's own pool, its counters zeroed by a node of the graph, so
+// graphs that replay at the same time share nothing and a graph's replay does
+// not depend on what the workspace held.  The tensor is kept until another
+// capture on the stream begins; the memory itself lives as long as its graph.
+std::map<std::pair<int, cudaStream_t>, std::pair<unsigned long long, torch::Tensor>> g_capture_ws;
+
+torch::Tensor capturable_workspace(WsKind kind, const torch::Device& dev, cudaStream_t stream, size_t bytes,
+                                   size_t counter_bytes) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  cudaError_t e = cudaStreamGetCaptureInfo(stream, &st, &id);
+  TORCH_CHECK(e == cudaSuccess, "cudaStreamGetCaptureInfo: ", cudaGetErrorString(e));
+  if (st == cudaStreamCaptureStatusNone) return workspace_for(kind, dev, stream, bytes);
+  std::lock_guard<std::mutex> lock(g_ws_mutex);
+  auto& slot = g_capture_ws[std::make_pair((int)dev.index(), stream)];
+  if (!slot.second.defined() || slot.first != id || (size_t)slot.second.numel() < bytes) {
+    slot.second = torch::empty({(int64_t)bytes}, torch::TensorOptions().dtype(torch::kUInt8).device(dev));
+    slot.first = id;
+    e = cudaMemsetAsync(slot.second.data_ptr(), 0, std::min(bytes, counter_bytes), stream);
+    TORCH_CHECK(e == cudaSuccess, "cudaMemsetAsync (workspace): ", cudaGetErrorString(e));
+  }
+  return slot.second;
+}
+
+// For calls without a workspace: report an earlier call's device-side failure.
+void check_device_status(const torch::Device& dev) {
+  std::lock_guard<std::mutex> lock(g_ws_mutex);
+  check_device_status_locked(dev);
 }
 
 torch::Tensor w4a16_workspace(const torch::Tensor& x, int64_t N) {
@@ -326,6 +359,200 @@ torch::Tensor gqa_decode_attention_paged(torch::Tensor q, torch::Tensor k_pages,
   return o;
 }
 
+// ------------------------------------------- rotary positions, 8-bit KV cache
+int dtype_of(const torch::Tensor& t, const char* name, bool fp32) {
+  if (t.scalar_type() == at::kBFloat16) return FOCAL_BF16;
+  if (t.scalar_type() == at::kHalf) return FOCAL_FP16;
+  TORCH_CHECK(fp32 && t.scalar_type() == at::kFloat, name, " has wrong dtype");
+  return FOCAL_FP32;
+}
+
+// [tokens, heads, D] rows: the last dimension contiguous, the others strided.
+void check_rows(const torch::Tensor& t, const char* name, const torch::Tensor& like) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.dim() == 3, name, " must have shape [T, H, D]");
+  TORCH_CHECK(t.size(2) <= 1 || t.stride(2) == 1, name, " must have a contiguous last dimension");
+  TORCH_CHECK(t.device() == like.device(), "all tensors must be on ", name, "'s device");
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " has wrong dtype");
+  TORCH_CHECK(t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX && t.size(2) <= INT32_MAX, "unsupported size");
+}
+
+// A dimension of one element has no stride to speak of.
+int64_t stride_of(const torch::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
+void check_inv_freq(const torch::Tensor& f, const torch::Tensor& like) {
+  check_tensor(f, "inv_freq", at::kDouble);
+  TORCH_CHECK(f.dim() == 1, "inv_freq must have shape [rot / 2]");
+  TORCH_CHECK(f.device() == like.device(), "inv_freq must be on the same device as the rows");
+  TORCH_CHECK(f.size(0) <= 65536, "unsupported size");
+}
+
+torch::Tensor rope(torch::Tensor x, torch::Tensor positions, torch::Tensor inv_freq, bool interleaved, double mscale,
+                   c10::optional<torch::Tensor> out) {
+  check_rows(x, "x", x);
+  const int dtype = dtype_of(x, "x", true);
+  check_inv_freq(inv_freq, x);
+  TORCH_CHECK(positions.is_cuda() && positions.device() == x.device(), "positions must be on the same device as x");
+  TORCH_CHECK(positions.is_contiguous(), "positions must be contiguous");
+  TORCH_CHECK(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong,
+              "positions has wrong dtype");
+  TORCH_CHECK(positions.dim() == 1 && positions.size(0) == x.size(0), "positions must have shape [T]");
+  const c10::cuda::CUDAGuard guard(x.device());
+  torch::Tensor y;
+  if (out.has_value()) {
+    y = *out;
+    check_rows(y, "out", x);
+    TORCH_CHECK(y.sizes() == x.sizes(), "out must have the shape of x");
+    at::assert_no_internal_overlap(y);
+    for (int d = 0; d < 2; ++d) TORCH_CHECK(y.size(d) <= 1 || y.stride(d) != 0, "out must not overlap itself");
+    if (y.data_ptr() == x.data_ptr()) {
+      TORCH_CHECK(stride_of(x, 0) == stride_of(y, 0) && stride_of(x, 1) == stride_of(y, 1),
+                  "in place, out must be x");
+    } else {
+      at::assert_no_partial_overlap(y, x);
+    }
+  } else {
+    y = torch::empty(x.sizes(), x.options());
+  }
+  raise_on(focal_rope(x.data_ptr(), y.data_ptr(), positions.data_ptr(), inv_freq.data_ptr<double>(), (int)x.size(0),
+                      (int)x.size(1), (int)x.size(2), 2 * (int)inv_freq.size(0), interleaved, mscale, dtype,
+                      positions.scalar_type() == at::kLong, stride_of(x, 0), stride_of(x, 1), stride_of(y, 0),
+                      stride_of(y, 1), current_stream()));
+  return y;
+}
+
+focal_kv8_cache kv8_cache_of(const torch::Tensor& k_pages, const torch::Tensor& v_pages, const torch::Tensor& k_scales,
+                             const torch::Tensor& v_scales, const torch::Tensor& rows, const char* rows_name) {
+  TORCH_CHECK(k_pages.scalar_type() == at::kFloat8_e4m3fn || k_pages.scalar_type() == at::kChar,
+              "k_pages has wrong dtype");
+  check_tensor(k_pages, "k_pages", k_pages.scalar_type());
+  check_tensor(v_pages, "v_pages", k_pages.scalar_type());
+  check_tensor(k_scales, "k_scales", at::kFloat);
+  check_tensor(v_scales, "v_scales", at::kFloat);
+  TORCH_CHECK(k_pages.dim() == 4, "k_pages must have shape [num_pages, Hkv, page_size, D]");
+  TORCH_CHECK(v_pages.sizes() == k_pages.sizes(), "v_pages must have the shape of k_pages");
+  const int64_t P = k_pages.size(0), H = k_pages.size(1), S = k_pages.size(2), D = k_pages.size(3);
+  TORCH_CHECK(P <= INT32_MAX && H <= INT32_MAX && S <= INT32_MAX && D <= INT32_MAX, "unsupported size");
+  TORCH_CHECK(k_scales.dim() == 3 && k_scales.size(0) == P && k_scales.size(1) == H && k_scales.size(2) == S / 16,
+              "k_scales must have shape [num_pages, Hkv, page_size / 16]");
+  TORCH_CHECK(v_scales.sizes() == k_scales.sizes(), "v_scales must have the shape of k_scales");
+  for (const auto* t : {&k_pages, &v_pages, &k_scales, &v_scales})
+    TORCH_CHECK(t->device() == rows.device(), "the cache must be on ", rows_name, "'s device");
+  focal_kv8_cache c{};
+  c.k_pages = k_pages.data_ptr();
+  c.v_pages = v_pages.data_ptr();
+  c.k_scales = k_scales.data_ptr<float>();
+  c.v_scales = v_scales.data_ptr<float>();
+  c.num_pages = (int)P;
+  c.num_kv_heads = (int)H;
+  c.page_size = (int)S;
+  c.head_dim = (int)D;
+  c.code = k_pages.scalar_type() == at::kChar ? FOCAL_INT8 : FOCAL_E4M3;
+  return c;
+}
+
+void check_tables(const torch::Tensor& block_table, const torch::Tensor& seq_lens, int64_t B,
+                  const torch::Tensor& like) {
+  check_tensor(block_table, "block_table", at::kInt);
+  check_tensor(seq_lens, "seq_lens", at::kInt);
+  TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) == B, "block_table must have shape [B, max_pages]");
+  TORCH_CHECK(seq_lens.dim() == 1 && seq_lens.size(0) == B, "seq_lens must have shape [B]");
+  TORCH_CHECK(block_table.device() == like.device() && seq_lens.device() == like.device(),
+              "all tensors must be on the same device");
+  TORCH_CHECK(B <= INT32_MAX && block_table.size(1) <= INT32_MAX, "unsupported size");
+}
+
+c10::optional<torch::Tensor> kv8_append(torch::Tensor k, torch::Tensor v, torch::Tensor k_pages, torch::Tensor v_pages,
+                                        torch::Tensor k_scales, torch::Tensor v_scales, torch::Tensor block_table,
+                                        torch::Tensor seq_lens, c10::optional<torch::Tensor> cu_new, int64_t max_new,
+                                        c10::optional<torch::Tensor> q, c10::optional<torch::Tensor> inv_freq,
+                                        bool interleaved, double mscale) {
+  check_rows(k, "k", k);
+  check_rows(v, "v", k);
+  focal_kv8_append_args a{};
+  a.dtype = dtype_of(k, "k", false);
+  const focal_kv8_cache cache = kv8_cache_of(k_pages, v_pages, k_scales, v_scales, k, "k");
+  TORCH_CHECK(v.sizes() == k.sizes(), "v must have the shape of k");
+  TORCH_CHECK(k.size(1) == cache.num_kv_heads && k.size(2) == cache.head_dim, "k must have shape [T, Hkv, D]");
+  TORCH_CHECK(seq_lens.dim() == 1, "seq_lens must have shape [B]");
+  const int64_t B = seq_lens.size(0), T = k.size(0);
+  check_tables(block_table, seq_lens, B, k);
+  TORCH_CHECK(max_new >= 0 && max_new <= INT32_MAX, "max_new must not be negative");
+  if (cu_new.has_value()) {
+    check_tensor(*cu_new, "cu_new", at::kInt);
+    TORCH_CHECK(cu_new->dim() == 1 && cu_new->size(0) == B + 1, "cu_new must have shape [B + 1]");
+    TORCH_CHECK(cu_new->device() == k.device(), "cu_new must be on k's device");
+    a.cu_new = cu_new->data_ptr<int32_t>();
+  }
+  if (inv_freq.has_value()) {
+    check_inv_freq(*inv_freq, k);
+    TORCH_CHECK(inv_freq->size(0) > 0, "inv_freq must not be empty");
+    a.inv_freq = inv_freq->data_ptr<double>();
+    a.rot = 2 * (int)inv_freq->size(0);
+  }
+  const c10::cuda::CUDAGuard guard(k.device());
+  c10::optional<torch::Tensor> turned;
+  if (q.has_value()) {
+    check_rows(*q, "q", k);
+    TORCH_CHECK(inv_freq.has_value(), "q needs inv_freq: it is only turned");
+    TORCH_CHECK(q->size(0) == T && q->size(2) == k.size(2), "q must have shape [T, Hq, D]");
+    turned = torch::empty(q->sizes(), q->options());
+    a.q = q->data_ptr();
+    a.q_out = turned->data_ptr();
+    a.Hq = (int)q->size(1);
+    a.q_token_stride = stride_of(*q, 0);
+    a.q_head_stride = stride_of(*q, 1);
+  }
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.k_token_stride = stride_of(k, 0);
+  a.k_head_stride = stride_of(k, 1);
+  a.v_token_stride = stride_of(v, 0);
+  a.v_head_stride = stride_of(v, 1);
+  a.block_table = block_table.data_ptr<int32_t>();
+  a.seq_lens = seq_lens.data_ptr<int32_t>();
+  a.B = (int)B;
+  a.T = (int)T;
+  a.max_new = (int)max_new;
+  a.max_pages_per_seq = (int)block_table.size(1);
+  a.interleaved = interleaved;
+  a.mscale = mscale;
+  check_device_status(k.device());
+  raise_on(focal_kv8_append(&a, &cache, current_stream()));
+  return turned;
+}
+
+torch::Tensor gqa_decode_attention_kv8(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages,
+                                       torch::Tensor k_scales, torch::Tensor v_scales, torch::Tensor block_table,
+                                       torch::Tensor seq_lens, int64_t max_seq_len, c10::optional<double> scale) {
+  TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+  TORCH_CHECK(q.is_contiguous(), "q must be contiguous");
+  const int dtype = dtype_of(q, "q", false);
+  TORCH_CHECK(q.dim() == 3 || q.dim() == 4, "q must have shape [B, Hq, D] or [B, T, Hq, D]");
+  const focal_kv8_cache cache = kv8_cache_of(k_pages, v_pages, k_scales, v_scales, q, "q");
+  const int64_t B = q.size(0), T = q.dim() == 4 ? q.size(1) : 1, Hq = q.size(-2), D = q.size(-1);
+  check_tables(block_table, seq_lens, B, q);
+  TORCH_CHECK(D == cache.head_dim, "k_pages must have shape [num_pages, Hkv, page_size, D]");
+  TORCH_CHECK(T <= INT32_MAX && Hq <= INT32_MAX && max_seq_len <= INT32_MAX && max_seq_len >= 1, "unsupported size");
+  const double sc = scale.has_value() ? *scale : 1.0 / std::sqrt((double)D);
+  const c10::cuda::CUDAGuard guard(q.device());
+  auto o = torch::empty(q.sizes(), q.options());
+  const cudaStream_t stream = current_stream();
+  const size_t bytes =
+      focal_kv8_decode_workspace_size((int)B, (int)T, (int)Hq, cache.num_kv_heads, (int)max_seq_len, (int)D);
+  void* ws = nullptr;
+  torch::Tensor ws_t;
+  if (bytes > 0) {
+    ws_t = capturable_workspace(kWsKv8, q.device(), stream, bytes,
+                                focal_kv8_decode_counter_bytes((int)B, (int)T, (int)Hq, cache.num_kv_heads));
+    ws = ws_t.data_ptr();
+  }
+  raise_on(focal_kv8_decode(q.data_ptr(), o.data_ptr(), &cache, block_table.data_ptr<int32_t>(),
+                            seq_lens.data_ptr<int32_t>(), (int)B, (int)T, (int)Hq, (int)block_table.size(1),
+                            (int)max_seq_len, (float)sc, dtype, ws, bytes, stream));
+  return o;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -338,6 +565,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("w4a16_gate_up_silu_tiled", &w4a16_gate_up_silu_tiled, "fused gate/up/SiLU on unit-tiled weights");
   m.def("dequant", &dequant, "fp32 dequantized weights (bit-identical to dequant_ref)");
   m.def("pack_int4", &pack_int4, "pack uint8 [N,K] nibbles into int32 [N,K/8]");
+  m.def("rope", &rope, "rotary positions", pybind11::arg("x"), pybind11::arg("positions"), pybind11::arg("inv_freq"),
+        pybind11::arg("interleaved") = false, pybind11::arg("mscale") = 1.0, pybind11::arg("out") = pybind11::none());
+  m.def("kv8_append", &kv8_append, "append keys and values to the 8-bit paged KV cache");
+  m.def("gqa_decode_attention_kv8", &gqa_decode_attention_kv8, "GQA decode attention over the 8-bit paged KV cache");
   m.def("gqa_decode_attention_paged", &gqa_decode_attention_paged, "paged variable-length GQA decode attention",
         pybind11::arg("q"), pybind11::arg("k_pages"), pybind11::arg("v_pages"), pybind11::arg("block_table"),
         pybind11::arg("seq_lens"), pybind11::arg("max_seq_len"), pybind11::arg("scale") = pybind11::none());

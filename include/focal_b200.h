@@ -251,6 +251,98 @@ int focal_gqa_decode_paged(const void* q, const void* k_pages, const void* v_pag
                            int page_size, int max_pages_per_seq, int max_seq_len, float scale, void* workspace,
                            size_t ws_bytes, cudaStream_t stream);
 
+/* ------------------------------------------------------ rotary positions ---
+ * y[t, h, :] = x[t, h, :] with its first `rot` dims turned by the angles
+ * positions[t] * inv_freq[i], i < rot / 2: pair i is dims (i, i + rot / 2), or
+ * (2i, 2i + 1) with `interleaved`, and (a, b) becomes mscale *
+ * (a cos - b sin, a sin + b cos).  The dims behind `rot` are copied.  Angles,
+ * cos and sin are 64-bit, rounded once to fp32; products and sums are fp32;
+ * one rounding to the output type.  New component (no reference counterpart).
+ *   x, y       [T, H, D] of dtype (focal_dtype), the last dimension contiguous;
+ *              strides in elements, multiples of 16 bytes; x and y 16-byte
+ *              aligned.  y == x with the same strides works in place; other
+ *              overlap is not allowed.  x's strides may be 0.
+ *   positions  [T] int32, or int64 with positions64; any value
+ *   inv_freq   fp64 [rot / 2], device memory: radians per position
+ * Contract: D % 8 == 0, 16 <= D <= 1024; rot % 16 == 0, 16 <= rot <= D. */
+typedef enum focal_dtype { FOCAL_BF16 = 0, FOCAL_FP16 = 1, FOCAL_FP32 = 2 } focal_dtype;
+
+int focal_rope(const void* x, void* y, const void* positions, const double* inv_freq, int T, int H, int D, int rot,
+               int interleaved, double mscale, int dtype, int positions64, int64_t x_token_stride,
+               int64_t x_head_stride, int64_t y_token_stride, int64_t y_head_stride, cudaStream_t stream);
+
+/* --------------------------------------------------- 8-bit paged KV cache ---
+ * K and V as 8-bit codes in pages [num_pages, num_kv_heads, page_size,
+ * head_dim], with one fp32 scale for every 16 consecutive tokens of a page and
+ * head, [num_pages, num_kv_heads, page_size / 16]; a code c stands for
+ * c * scale.  Page j of sequence b is block_table[b * max_pages_per_seq + j].
+ * Contract: head_dim 64 or 128; page_size 16, 32 or a multiple of 64; all four
+ * arrays 16-byte aligned.  New components (the reference has no cache). */
+typedef enum focal_code { FOCAL_E4M3 = 0, FOCAL_INT8 = 1 } focal_code;
+
+typedef struct focal_kv8_cache {
+  void* k_pages;
+  void* v_pages;
+  float* k_scales;
+  float* v_scales;
+  int num_pages, num_kv_heads, page_size, head_dim;
+  int code; /* focal_code */
+} focal_kv8_cache;
+
+/* Append each sequence's new tokens: sequence b's are rows cu_new[b] ..
+ * cu_new[b + 1] - 1 of k and v (without cu_new: max_new rows each, in order),
+ * and become its last positions, seq_lens[b] - n .. seq_lens[b] - 1 (seq_lens
+ * counts them already).  With rot > 0, k is turned by its positions first (see
+ * focal_rope), and so is q into q_out, both from the same tokens.
+ *
+ * For the new rows of a block of 16 tokens and a head, amax = max |x|;
+ *   e4m3: need = the smallest power of two >= amax / 448; int8: amax / 127
+ *   scale = max(old scale, need), where the old scale counts as 0 if the
+ *   block's first row is among the new; code = nearest-even(x / scale).
+ * If the scale grows, the codes of the block's older rows are moved to it.
+ * Rows behind a sequence's last token are left as they were.  Infinities
+ * saturate; NaN becomes e4m3's NaN or int8's 0.  All the rows appended to a page
+ * must belong to one sequence of the call.
+ *
+ * Contract: n <= max_new for every sequence (max_new, on the host, sizes the
+ * launch); k, v, q [T, heads, head_dim] of dtype bf16 or fp16 with strides in
+ * elements (multiples of 16 bytes), 16-byte aligned; q_out [T, Hq, head_dim]
+ * contiguous; rot 0 or a multiple of 16 up to head_dim; Hq = 0 without q.
+ * A length, cu_new entry or page id out of range sets device status 3, and
+ * nothing is written for that sequence (or block). */
+typedef struct focal_kv8_append_args {
+  const void *k, *v, *q;
+  void* q_out;
+  const int32_t *block_table, *seq_lens, *cu_new;
+  const double* inv_freq;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride, q_token_stride, q_head_stride;
+  int B, T, max_new, Hq, max_pages_per_seq, rot, interleaved, dtype;
+  double mscale;
+} focal_kv8_append_args;
+
+int focal_kv8_append(const focal_kv8_append_args* args, const focal_kv8_cache* cache, cudaStream_t stream);
+
+/* Attention of T query tokens per sequence, its last T positions, over the
+ * cache: query token t of sequence b sees positions < seq_lens[b] - T + 1 + t.
+ *   q, o [B, T, Hq, head_dim] of dtype (bf16 or fp16), contiguous
+ * fp32 scores, softmax and accumulation; split over the positions with a
+ * log-sum-exp combine in split order.  A query that sees no position gives 0.
+ * seq_lens[b] is 0 .. max_seq_len <= max_pages_per_seq * page_size (block
+ * table entries and rows past a sequence's end are not read as data).
+ * Contract: Hq % num_kv_heads == 0, Hq / num_kv_heads <= 16, 1 <= T <= 16.
+ *
+ * Workspace: focal_kv8_decode_workspace_size() bytes, 256-byte aligned; its
+ * first focal_kv8_decode_counter_bytes() bytes must be zero before the first
+ * call, and every call that returns FOCAL_OK leaves them zero again.  Calls that
+ * share a workspace must be ordered.  A page id or length out of range sets
+ * device status 3 and is clamped (the output is then not meaningful). */
+size_t focal_kv8_decode_workspace_size(int B, int T, int Hq, int Hkv, int max_seq_len, int D);
+size_t focal_kv8_decode_counter_bytes(int B, int T, int Hq, int Hkv);
+
+int focal_kv8_decode(const void* q, void* o, const focal_kv8_cache* cache, const int32_t* block_table,
+                     const int32_t* seq_lens, int B, int T, int Hq, int max_pages_per_seq, int max_seq_len,
+                     float scale, int dtype, void* workspace, size_t ws_bytes, cudaStream_t stream);
+
 /* ------------------------------------------------------------ diagnostics ---
  * Device-side status word of the current device: 0 while every kernel's
  * bounded waits have completed; otherwise 1 (a pipeline wait gave up), 2 (a

@@ -31,7 +31,6 @@ namespace focal {
 namespace kv8 {
 
 constexpr int kAppendWarps = 8;
-constexpr float kMinScale = 1.17549435e-38f;  // 2^-126: scales stay normal numbers
 
 struct AppendParams {
   const void *k, *v, *q;

@@ -11,12 +11,35 @@ namespace focal {
 namespace kv8 {
 
 constexpr int kGroup = 16;  // consecutive tokens of a page and KV head that share a scale
+constexpr float kMinScale = 1.17549435e-38f;  // 2^-126: scales stay normal numbers
 
 // Two e4m3 codes (low byte first) as f16x2; every e4m3 value is exact in f16.
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t c) {
   uint32_t r;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(c));
   return r;
+}
+
+// Four codes of a word (bytes 0 .. 3) as two f16x2 words of the numbers they
+// are, all exact in f16: bytes (0, 1) and (2, 3), or with `STRIDED` bytes (0, 2)
+// and (1, 3).  int8: the code with its sign bit flipped, under f16 1024's
+// exponent, reads 1024 + 128 + c; one subtraction leaves c.
+template <bool INT8, bool STRIDED>
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (INT8) {
+    w ^= 0x80808080u;
+    const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
+    const uint32_t a = prmt(w, 0x64646464u, STRIDED ? 0x4240u : 0x4140u);
+    const uint32_t b = prmt(w, 0x64646464u, STRIDED ? 0x4341u : 0x4342u);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    if (STRIDED) w = prmt(w, 0u, 0x3120u);
+    lo = e4m3x2_to_f16x2(static_cast<uint16_t>(w));
+    hi = e4m3x2_to_f16x2(static_cast<uint16_t>(w >> 16));
+  }
 }
 
 // Two floats as e4m3 codes (`lo` in the low byte), nearest even, saturating at
@@ -45,10 +68,22 @@ __device__ __forceinline__ void rope_turn(float& a, float& b, float2 cs) {
   a = u;
 }
 
-template <typename T>
-__device__ __forceinline__ float to_f32(T x) {
-  return static_cast<float>(x);
+// D = A(16x16, row) * B(16x8, col) + C, f16 inputs, fp32 accumulate.
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+
+// The transpose of an 8x8 tile of 16-bit values, two of a row in each lane.
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);  // one 32-bit word, one rounding each
 template <>

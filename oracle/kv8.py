@@ -88,14 +88,15 @@ def gather(codes, scales, block_table, b, n):
 
 
 def attention(q, cache, block_table, seq_lens, scale=None):
-    """(o, a, s): o [B, T, Hq, D] float64; a = sum of p |v| and s = the largest
-    scale * sum |q| |k| of each row, for error bounds."""
+    """(o, a, s, w): o [B, T, Hq, D] float64, and for error bounds a = sum of p |v|,
+    s = the largest scale * sum |q| |k| of each row, and w = its number of positions
+    times the largest V scale times the largest V code."""
     B, T, Hq, D = q.shape
     H = cache[0].shape[1]
     grp = Hq // H
     scale = D ** -0.5 if scale is None else scale
     o = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
-    a, s = torch.zeros_like(o), torch.zeros_like(o[..., :1])
+    a, s, w = torch.zeros_like(o), torch.zeros_like(o[..., :1]), torch.zeros_like(o[..., :1])
     for b in range(B):
         n = int(seq_lens[b])
         if n == 0:
@@ -110,5 +111,8 @@ def attention(q, cache, block_table, seq_lens, scale=None):
             p = torch.softmax(qg @ k[:, :m].transpose(1, 2) * scale, -1)
             o[b, t] = (p @ v[:, :m]).view(Hq, D)
             a[b, t] = (p @ v[:, :m].abs()).view(Hq, D)
+            used = block_table[b, :-(-m // cache[1].shape[2])].long()
+            top = cache[1][used].abs().nan_to_num(0.0).amax() * cache[3][used].nan_to_num(0.0).amax()
+            w[b, t] = m * top
             s[b, t] = (qg.abs() @ k[:, :m].abs().transpose(1, 2) * scale).amax(-1).view(Hq, 1)
-    return o, a, s
+    return o, a, s, w

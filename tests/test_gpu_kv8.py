@@ -251,14 +251,18 @@ def test_append_refusals_on_the_device(cuda):
 
 
 # --------------------------------------------------------------- attention
-def attention_tolerance(o, a, s, dtype, D):
-    """Scores: D products and sums and a handful of scalings in fp32, (D + 16) 2^-24 of
-    scale * sum |q| |k| at most; a weight is off by twice that (numerator and sum), by half
-    a step of the 16-bit weight (2^-11) and by the fp32 exponentials and sums, 2^-18;
-    what a weight's error moves is at most its share of sum p |v|.  Then the output's
-    rounding."""
-    noise = (2 * (D + 16) * 2.0 ** -24 * s + 2.0 ** -11 + 2.0 ** -18) * a
-    return noise + (o.abs() + noise) * (torch.finfo(dtype).eps / 2) + 2.0 ** -25 * a + 2.0 ** -24 * (dtype == FP16)
+def attention_tolerance(bounds, dtype, D):
+    """`bounds` as ok.attention gives them.  Scores: D products and sums and a handful of
+    scalings in fp32, (D + 16) 2^-24 of scale * sum |q| |k| at most; a weight is off by
+    twice that (numerator and sum), by half a step of the 16-bit weight (2^-11) and by
+    the fp32 exponentials and sums, 2^-18; what a weight's error moves is at most its
+    share of sum p |v|.  A weight enters as f16(2^15 p vs / R) with R at most twice the
+    largest V scale: below f16's normal numbers that is off by up to 2^-25, which is
+    2^-40 R / vs of the weight of the maximum, so 2^-39 times the largest V scale and
+    code for each position.  Then the output's rounding (and fp16's smallest subnormal's half)."""
+    o, a, s, w = bounds
+    noise = (2 * (D + 16) * 2.0 ** -24 * s + 2.0 ** -11 + 2.0 ** -18) * a + 2.0 ** -39 * w
+    return noise + (o.abs() + noise) * (torch.finfo(dtype).eps / 2) + 2.0 ** -25 * (dtype == FP16)
 
 
 def random_cache(pages, H, page_size, D, code, device, seed, wild=True):
@@ -294,9 +298,9 @@ def check_attention(cuda, B, T, Hq, H, D, page_size, lens, max_len, code, dtype,
     spoil(cache, table.cpu(), lens, page_size)
     q = (torch.randn(B, T, Hq, D, device=cuda, generator=gen(cuda, seed + 1)) * q_gain).to(dtype)
     got = F.gqa_decode_attention_kv8(q[:, 0] if T == 1 else q, cache, table, ints(lens, cuda), max_len, scale)
-    o, a, s = ok.attention(q, doubles(cache), table.cpu(), lens, scale)
-    err = (got.view(q.shape).double() - o).abs()
-    tol = attention_tolerance(o, a, s, dtype, D)
+    bounds = ok.attention(q, doubles(cache), table.cpu(), lens, scale)
+    err = (got.view(q.shape).double() - bounds[0]).abs()
+    tol = attention_tolerance(bounds, dtype, D)
     assert torch.all(torch.isfinite(got))
     assert torch.all(err <= tol), float((err / tol.clamp(min=1e-300)).max())
     assert status() == 0
@@ -347,8 +351,8 @@ def test_attention_scales_of_all_sizes(cuda):
     q = torch.randn(1, 1, 4, D, device=cuda, generator=gen(cuda, 2)).to(BF16)
     for m in (n, 16, 32, 96, 160, 176, 48):
         got = F.gqa_decode_attention_kv8(q, cache, table, ints([m], cuda), n)
-        o, a, s = ok.attention(q, doubles(cache), table.cpu(), [m])
-        assert torch.all((got.double() - o).abs() <= attention_tolerance(o, a, s, BF16, D)), m
+        bounds = ok.attention(q, doubles(cache), table.cpu(), [m])
+        assert torch.all((got.double() - bounds[0]).abs() <= attention_tolerance(bounds, BF16, D)), m
     zero = torch.zeros_like(cache.v_scales)
     got = F.gqa_decode_attention_kv8(q, F.Kv8Cache(*cache[:3], zero), table, ints([n], cuda), n)
     assert torch.all(got == 0)
@@ -464,8 +468,8 @@ def decode_run(cuda, code, interleaved, steps, T, prompt, capture=False):
             out = F.decode_attention_kv8(*split(x), cache, table, lens, max(final), f, interleaved)
     pos = (lens[:, None].long() - T + torch.arange(T, device=cuda)).flatten()
     turned = F.rope(split(x)[0], pos, f, interleaved).view(B, T, Hq, D)
-    o, a, s = ok.attention(turned, doubles(cache), table.cpu(), final)
-    return out.view(B, T, Hq, D), o, attention_tolerance(o, a, s, BF16, D)
+    bounds = ok.attention(turned, doubles(cache), table.cpu(), final)
+    return out.view(B, T, Hq, D), bounds[0], attention_tolerance(bounds, BF16, D)
 
 
 @pytest.mark.parametrize("code", [E4M3, INT8])

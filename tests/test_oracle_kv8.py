@@ -84,7 +84,7 @@ def test_append_then_attention_near_unquantised():
         assert torch.all((back - x).abs() <= step[..., None] * 8)
         assert torch.all((back[:16] - x[:16]).abs() <= step[:16, :, None] * 0.5000001)
     q = torch.randn(1, 2, 4, D, generator=g, dtype=torch.float64)
-    o, a, s = ok.attention(q, cache, table, [n])
+    o, _, _, _ = ok.attention(q, cache, table, [n])
     want = torch.nn.functional.scaled_dot_product_attention(
         q.transpose(1, 2), ok.gather(cache[0], cache[2], table, 0, n)[None].repeat_interleave(2, 1),
         ok.gather(cache[1], cache[3], table, 0, n)[None].repeat_interleave(2, 1),
@@ -94,5 +94,5 @@ def test_append_then_attention_near_unquantised():
 
 def test_attention_rows_that_see_nothing_are_zero():
     cache = [torch.ones(1, 1, 16, 64).double() for _ in "kv"] + [torch.ones(1, 1, 1).double() for _ in "kv"]
-    o, _, _ = ok.attention(torch.ones(2, 4, 1, 64), cache, torch.zeros(2, 1, dtype=torch.int64), [2, 0])
+    o, _, _, _ = ok.attention(torch.ones(2, 4, 1, 64), cache, torch.zeros(2, 1, dtype=torch.int64), [2, 0])
     assert torch.all(o[0, :2] == 0) and torch.all(o[0, 2:] == 1) and torch.all(o[1] == 0)

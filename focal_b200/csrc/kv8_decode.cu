@@ -6,76 +6,110 @@
 // New component (the reference has no attention code).
 //
 // Bound: HBM, by the codes (2 D bytes per position and KV head); the codes are
-// half of a bf16 cache's bytes, so a CTA has half the time per position and the
-// work per code counts.  Split-KV: one CTA takes one (sequence, KV head, up to 16
-// query rows) and a contiguous range of 64-position tiles.
-//  * warp kWarps (producer) looks up the pages and streams K and V tiles (64
-//    positions x D bytes, swizzled) and their 4 + 4 scales by TMA into a ring;
-//  * each of the kWarps consumer warps takes every kWarps-th tile for itself, so
-//    warps never wait for one another within a tile and the softmax's
-//    reductions are paid once per 64 positions;
-//  * the products are transposed: S^T = K Q^T and O^T = V^T P^T.  The 16-row side
+// half of a bf16 cache's bytes, so an SM has half the time per position and the
+// work per code counts.
+//  * All tiles (kTile positions of one segment: a sequence, a KV head and up to 16
+//    query rows) of all sequences form one flat order, which is cut into
+//    equal ranges, one per CTA, and these into one per warp.  Lengths that
+//    differ, and numbers of segments that do not divide the SMs, cost nothing.
+//    Where a segment lies in several warps or CTAs its parts are joined by their
+//    log-sum-exp, in the flat order: in shared memory, then by the last CTA to arrive.
+//  * Every warp streams its own tiles through a ring of its own: it issues the TMA
+//    boxes of a tile's K and V (swizzled) and the copies of its scales, kRing tiles
+//    ahead, into the slot it has just read.  No warp waits for another before
+//    the end, and a late box holds up one ring only.
+//  * The products are transposed: S^T = K Q^T and O^T = V^T P^T.  The 16-row side
 //    of mma.sync m16n8k16 holds positions and dims, its 8-column side the query rows
 //    (T * Hq / Hkv, 8 or 16 of them), which halves the products that 4 or 8
 //    query rows would need as the 16-row side.  (A tcgen05 tile's 64 or 128 rows
 //    would be as empty, and its operands would have to be converted through
 //    shared memory first.)
-//  * codes become f16 exactly.  K's words are read 16 bytes a lane as they lie: the
+//  * Codes become f16 exactly.  K's words are read 16 bytes a lane as they lie: the
 //    sum over dims may run in any order, so q is loaded in the same order.  V's
 //    come through ldmatrix.trans as pairs of dims, and the two bytes of a pair
-//    go to the two halves of the 16 rows;
+//    go to the two halves of the 16 rows.
 //  * q rows are scaled by a power of two to below 2^15, so bf16's range fits
-//    f16 and what sinks below f16's smallest number is 2^-38 of the row's largest;
-//  * a weight enters P V as f16(2^15 p vs / R): 2^15 moves it up in f16's range
+//    f16 and what sinks below f16's smallest number is 2^-38 of the row's largest.
+//  * A weight enters P V as f16(2^15 p vs / R): 2^15 moves it up in f16's range
 //    (p >= 2^-29 keeps f16's 11 bits), vs is its block's V scale and R the smallest power
 //    of two >= the V scales seen by the warp so far, so vs / R <= 1; when R
-//    grows the accumulators are rescaled as they are when the maximum grows;
-//  * splits are joined by the last CTA to finish, in split order.
+//    grows the accumulators are rescaled as they are when the maximum grows.
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 
 #include "kv8_common.cuh"
 
 namespace focal {
 namespace kv8 {
 
-constexpr int kTile = 64;     // positions per stage
-constexpr int kWarps = 8;     // consumer warps
-constexpr int kDecodeThreads = 32 * (kWarps + 1);
-constexpr int kStages = 12;
+constexpr int kTile = 64;  // positions of a tile
+constexpr int kTileBits = 6;
+constexpr int kBlocks = kTile / kGroup;  // blocks of the cache (scales) in a tile
+constexpr int kRing = 2;                 // tiles of a warp's ring
+// Warps of a CTA: what fits into shared memory; for head_dim 64 (half the bytes
+// a tile, but the same softmax) as many as fit into the registers.
+__host__ __device__ constexpr int warps_of(int D) { return D == 128 ? 7 : 12; }
+constexpr int kMaxWarps = warps_of(64) > warps_of(128) ? warps_of(64) : warps_of(128);
 constexpr int kMaxQueryTokens = 16;
 constexpr int kMaxGroup = 16;
-constexpr int kRowsPerCta = 16;
-constexpr int kMaxSplits = 128;
+constexpr int kRowsPerCta = 16;  // query rows of a segment
+constexpr int kMaxCtas = 256;
 constexpr int kCounterBytes = 256;  // granularity of the counters' region
-constexpr int kCombineBatch = 8;
+constexpr int kBatch = 16;  // records whose loads a join has in flight
+constexpr int kJoin = 4;    // ways that many records are shared out
 constexpr float kWeightUp = 32768.f;
+
+// n / d for 0 <= n < 2^31 by a product and a shift (Granlund and Montgomery, 1994).
+struct FastDiv {
+  uint32_t mul, shift;
+  void set(uint32_t d) {
+    shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
+  }
+};
 
 struct DecodeParams {
   const void* q;
   void* o;
   const float *k_scales, *v_scales;
   const int32_t *block_table, *seq_lens;
-  float* part_o;   // [BHC][splits][kRowsPerCta][D]
-  float* part_ml;  // [BHC][splits][kRowsPerCta][2]
-  unsigned int* counters;
+  float* first_rec;        // [CTA][warp] records of portions that a warp left behind for its next segment
+  float* cta_rec;          // [CTA][2] records of segments that come from, or go on into, another CTA
+  unsigned int* counters;  // [B][Hkv][chunks]
   int* status;
-  int T, Hq, Hkv, grp, chunks, num_pages, page_size, max_pages, max_len;
-  int tiles_per_split, splits;
+  int B, T, Hq, Hkv, grp, chunks, num_pages, page_size, max_pages, max_len;
+  // By segments: segs of them, `ways` CTAs each (0: more segments than CTAs) with
+  // `per` tiles each.  With `decide`, the kernel may share the tiles out evenly
+  // instead, or stack `stack` whole segments on a CTA.
+  int segs, ways, per, stack, decide;
   float scale_log2;
+  FastDiv by_hc, by_chunks, by_grp, by_page, by_grid, by_ways;
+};
+
+// A part of a segment: the segment's number (-1: none) and the flat range of all of it.
+struct Portion {
+  int seg, begin, end;
 };
 
 template <int D>
 struct Smem {
+  static constexpr int kWarps = warps_of(D);
   static constexpr int kTileBytes = kTile * D;
-  static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kRing = kStages * kStageBytes;
-  static constexpr int kScales = kRing;                    // [stage][K 4, V 4] fp32
-  static constexpr int kMl = kScales + kStages * 32;       // [warp][row][2]
-  static constexpr int kFlag = kMl + kWarps * kRowsPerCta * 8;
-  static constexpr int kBars = kFlag + 16;
-  static constexpr int kBytes = 1024 + kBars + 2 * kStages * 8;
-  static_assert(kWarps * kRowsPerCta * D * 4 <= kRing, "the warps' partial outputs alias the ring");
+  static constexpr int kSlotBytes = 2 * kTileBytes;
+  static constexpr int kWarpBytes = kRing * kSlotBytes;  // a warp's ring, and at the end its last portion's record
+  static constexpr int kPortions = kWarps * kWarpBytes;  // Portion [warp][first, last]
+  static constexpr int kParts = kPortions + kWarps * 2 * 12;  // Portion [2]: what cta_rec got
+  static constexpr int kLast = kParts + 2 * 12;               // int [2]
+  static constexpr int kBars = (kLast + 8 + 7) / 8 * 8;       // [warp][slot]
+  static constexpr int kBytes = 1024 + kBars + kWarps * kRing * 8;
+  static constexpr int kRow = D + 8;  // floats of a record's row; 8 more than needed, for fewer bank conflicts
+  static_assert(kRowsPerCta * (kRow + 2) * 4 <= kWarpBytes, "a record aliases its warp's ring");
+  static_assert(kRowsPerCta * kJoin * (D + 4) * 4 <= kPortions, "a join's partial results alias the rings");
   static_assert(kBytes <= 227 * 1024, "shared memory per CTA");
   // byte of 16-byte chunk c of row r in a tile as a TMA box with rows of D bytes leaves it (swizzle over D bytes)
   static __device__ __forceinline__ uint32_t at(int r, int c) {
@@ -94,228 +128,383 @@ __device__ __forceinline__ void store4(T* p, float4 v) {
   *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
 }
 
+// 2^e for e <= 127; 0 below the normal numbers
+__device__ __forceinline__ float exp2_int(int e) {
+  return e < -126 ? 0.f : __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+// x / n by an estimate that is made exact; 0 <= x, 0 < n, x / n < 2^20
+__device__ __forceinline__ int div_estimated(int x, int n) {
+  int q = __float2int_rz(__fdividef(static_cast<float>(x), static_cast<float>(n)));
+  while (q * n > x) --q;
+  while (x - q * n >= n) ++q;
+  return q;
+}
+
 template <typename T, int D, bool INT8, int NT>
-__global__ void __launch_bounds__(kDecodeThreads, 1)
+__global__ void __launch_bounds__(32 * warps_of(D))
     decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                   const DecodeParams p) {
   using S = Smem<D>;
+  constexpr int kWarps = S::kWarps, kDecodeThreads = 32 * kWarps;
   constexpr int kSteps = D / 16;   // k steps of K Q^T
   constexpr int kChunks = D / 16;  // 16-dim row blocks of V^T P^T
+  constexpr int kRows = 8 * NT;
+  constexpr int kRow = S::kRow;
+  constexpr int kLane = D / 32;
+  using LaneVec = typename std::conditional<D == 128, float4, float2>::type;
+  constexpr int kRec = kRows * (kRow + 2);  // floats of a record: [row][kRow], [row]{maximum, sum}
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* sm = smem_raw + (base - raw);
-  const uint32_t full_bar = base + S::kBars, empty_bar = full_bar + kStages * 8;
-
-  const int split = blockIdx.x;
-  const int bh = blockIdx.y;  // b * Hkv + KV head
-  const int b = bh / p.Hkv, kvh = bh - b * p.Hkv;
-  const int bhc = bh * p.chunks + blockIdx.z;
-  const int row0 = blockIdx.z * kRowsPerCta;  // first of this CTA's rows among the T * grp
-  const int rows = min(kRowsPerCta, p.T * p.grp - row0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool small_pages = p.page_size < kTile;
+  const uint32_t ring = base + warp * S::kWarpBytes;
+  const uint32_t full_bar = base + S::kBars + warp * (kRing * 8);
+  Portion* portions = reinterpret_cast<Portion*>(sm + S::kPortions) + 2 * warp;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(full_bar + 8 * s, small_pages ? 9 : 1);  // small pages: 8 lanes bring a scale each
-      mbar_init(empty_bar + 8 * s, 1);
-    }
+  if (lane == 0) {  // a warp's barriers are its own
+    for (int i = 0; i < kRing; ++i) mbar_init(full_bar + 8 * i, 1);
     fence_barrier_init();
-    griddep_launch_dependents();
+    portions[0].seg = portions[1].seg = -1;
+    if (warp == 0) {
+      prefetch_tensormap(&tmap_k);
+      prefetch_tensormap(&tmap_v);
+    }
   }
-  __syncthreads();
-  if (warp == kWarps && lane == 0) {
-    prefetch_tensormap(&tmap_k);
-    prefetch_tensormap(&tmap_v);
+  {  // the block table into L2, a line a thread, while the lengths are on their way
+    const size_t at = ((size_t)blockIdx.x * kDecodeThreads + threadIdx.x) * 32;
+    if (at < (size_t)p.B * p.max_pages) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.block_table + at));
   }
+  __syncwarp();
+  griddep_launch_dependents();
   griddep_wait();
 
-  int len = p.seq_lens[b];
-  if (len < 0 || len > p.max_len) {
-    if (threadIdx.x == 0 && split == 0) set_status(p.status, kDevBadIndex);
-    len = len < 0 ? 0 : p.max_len;
+  // ---- the flat order of all tiles: sequences, then their segments (KV head, rows
+  // chunk), then a segment's tiles.  CTA c takes tiles f0 .. f1 - 1, this warp
+  // nj of them from g0 on.
+  const int hc = p.Hkv * p.chunks;  // segments of a sequence
+  auto tiles_of = [](int len) { return (len + kTile - 1) / kTile; };
+  auto len_of = [&](int b) { return min(max(p.seq_lens[b], 0), p.max_len); };
+  auto checked_len = [&](int b) {  // 0 behind the last sequence
+    int n = 0;
+    if (b < p.B) {
+      n = p.seq_lens[b];
+      if (n < 0 || n > p.max_len) {
+        set_status(p.status, kDevBadIndex);
+        n = n < 0 ? 0 : p.max_len;
+      }
+    }
+    return n;
+  };
+
+  // ---- this CTA's tiles: f0 .. f1 - 1 of the flat order.
+  // By segments, every CTA has one segment's part (f counts within its sequence):
+  // nothing to locate, often nothing to join, but the longest segment sets the
+  // time.  Evenly, every CTA has `per` tiles of all.  In SM cycles: HBM needs
+  // kHbm for each of all tiles, a CTA kOwn for each of its own (measured with 128
+  // CTAs at work), a join and what goes with it 2000 and 3500.
+  constexpr float kHbm = D == 128 ? 4.8f : 2.4f;
+  constexpr int kOwn = (D == 128 ? 560 : 320) * (NT == 2 ? 5 : 4) / 4 * (INT8 ? 9 : 8) / 8;
+  const int cta = blockIdx.x;
+  int ways = p.ways, per = p.per;
+  int total = 0, len32 = 0;
+  bool empty = false;
+  if (p.decide) {
+    len32 = checked_len(lane);  // the first 32 sequences stay in registers
+    empty = lane < p.B && len32 == 0;
+    int top = tiles_of(len32);  // tiles of one segment of the longest sequence
+    total = top;
+    for (int b = lane + 32; b < p.B; b += 32) {
+      const int n = checked_len(b);
+      empty |= n == 0;
+      total += tiles_of(n);
+      top = max(top, tiles_of(n));
+    }
+    empty = __any_sync(0xffffffffu, empty);
+    total = __reduce_add_sync(0xffffffffu, total) * hc;
+    top = __reduce_max_sync(0xffffffffu, top);
+    const int hbm = static_cast<int>(kHbm * total), even = max(4, p.by_grid(total + gridDim.x - 1));
+    const int evenly = max(hbm, kOwn * even) + 3500;
+    if (ways > 0) {
+      if (top <= kWarps * 3 / 2) ways = 1;
+      const int part = ways == 1 ? top : p.by_ways(top + ways - 1);
+      per = max(part, 1);
+      if (max(hbm, kOwn * part) + (ways > 1 ? 2000 : 0) > evenly) ways = 0;
+    } else {
+      per = 0;
+      if (total == p.segs * top && max(hbm, kOwn * p.stack * top) <= evenly) per = p.stack * top;
+    }
+    if (ways == 0 && (p.ways > 0 || per == 0)) per = even;
   }
-  // row r of the output (and of q)
-  auto row_at = [&](int r) {
-    const int t = r / p.grp;
+  int f0 = 0, f1 = 0, cb = 0, seq_begin = 0, clen = 0, first_cta = 0;
+  if (ways > 0) {
+    const int seg = ways == 1 ? cta : p.by_ways(cta);
+    if (seg < p.segs) {
+      first_cta = seg * ways;
+      cb = p.by_hc(seg);
+      clen = checked_len(cb);
+      const int n = tiles_of(clen), begin = (seg - cb * hc) * n;
+      f0 = begin + min((cta - first_cta) * per, n);
+      f1 = min(f0 + per, begin + n);
+    }
+  } else {
+    f0 = min(cta * per, total);
+    f1 = min(f0 + per, total);
+  }
+  // the CTAs that have a segment (of which this one has a part)
+  auto ctas_of = [&](const Portion& s, int& c0) {
+    c0 = ways ? first_cta : div_estimated(s.begin, per);
+    return ways ? div_estimated(s.end - s.begin + per - 1, per) : div_estimated(s.end - 1, per) - c0 + 1;
+  };
+  const int wper = (f1 - f0) / kWarps, wmore = (f1 - f0) - wper * kWarps;
+  const int g0 = f0 + wper * warp + min(warp, wmore);
+  const int nj = wper + (warp < wmore ? 1 : 0);
+
+  // row r (of T * grp) of sequence b and KV head kvh
+  auto row_at = [&](int b, int kvh, int r) {
+    const int t = p.by_grp(r);
     return (((long long)b * p.T + t) * p.Hq + kvh * p.grp + (r - t * p.grp)) * D;
   };
   T* o = static_cast<T*>(p.o);
-  const int tiles = (len + kTile - 1) / kTile;
-  const int splits = (tiles + p.tiles_per_split - 1) / p.tiles_per_split;
-  const int t0 = split * p.tiles_per_split;
-  const int nt = min(tiles, t0 + p.tiles_per_split) - t0;
-  if (len == 0 && split == 0) {
-    for (int e = threadIdx.x; e < rows * (D / 4); e += kDecodeThreads)
-      store4(o + row_at(row0 + e / (D / 4)) + e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+  // sequences without positions have no tiles
+  if (ways > 0) {
+    if (clen == 0 && cta == first_cta && cta < p.segs * ways) {
+      const int sl = (ways == 1 ? cta : p.by_ways(cta)) - cb * hc, kvh = p.by_chunks(sl), row0 = (sl - kvh * p.chunks) * kRowsPerCta;
+      for (int e = threadIdx.x; e < min(kRowsPerCta, p.T * p.grp - row0) * (D / 4); e += kDecodeThreads)
+        store4(o + row_at(cb, kvh, row0 + e / (D / 4)) + e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+    }
+  } else if (empty) {
+    for (int b = cta; b < p.B; b += gridDim.x)
+      if (len_of(b) == 0)
+        for (int e = threadIdx.x; e < p.T * p.Hq * (D / 4); e += kDecodeThreads)
+          store4(o + (long long)b * p.T * p.Hq * D + 4 * e, make_float4(0.f, 0.f, 0.f, 0.f));
   }
-  if (nt <= 0) return;  // a split past this sequence's end: nothing to do, no arrival
+  if (f0 == f1) return;
 
-  if (warp == kWarps) {
-    // ------------------------------------------------------------- producer
-    const int box = small_pages ? p.page_size : kTile;  // rows of a box
-    const int32_t* bt = p.block_table + (size_t)b * p.max_pages;
-    const int first_page = (int)((long long)t0 * kTile / p.page_size), last_page = (len - 1) / p.page_size;
-    const int groups = p.page_size / kGroup;
-    const uint64_t pol = l2_policy_evict_first();
-    int chunk = -1, my_id = 0;
-    bool ok = true;
-    for (int i = 0; i < nt; ++i) {
-      const int slot = i % kStages;
-      if (i >= kStages) {
-        bool w = true;
-        if (lane == 0) w = mbar_wait_bounded(empty_bar + 8 * slot, ((i / kStages) - 1) & 1);
-        if (!__shfl_sync(0xffffffffu, w ? 1 : 0, 0)) {
-          ok = false;
-          break;
-        }
+  // ---- the sequence of this warp's first tile: it begins at flat tile seq_begin
+  if (ways == 0 && nj > 0) {
+    const int at = p.by_hc(g0);  // in the tiles of one segment of each sequence
+    int sum = 0, b0 = 0, n = len32;
+    while (true) {
+      int incl = tiles_of(n);
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, x);
+        if (lane >= x) incl += y;
       }
-      const uint32_t fb = full_bar + 8 * slot;
-      const uint32_t dst = base + slot * S::kStageBytes;
-      const uint32_t sc = base + S::kScales + slot * 32;
-      const int pos = (t0 + i) * kTile;
-      const int page = pos / p.page_size;  // index in the sequence of the tile's first page
-      // 32 block-table entries at a time; a tile's pages never straddle two such loads
-      const int c = (page - first_page) >> 5;
-      if (c != chunk) {
-        chunk = c;
-        const int j = first_page + 32 * c + lane;
-        my_id = j <= last_page ? bt[j] : 0;
-        if (my_id < 0 || my_id >= p.num_pages) {
-          set_status(p.status, kDevBadIndex);
-          my_id = 0;
-        }
+      const unsigned int found = __ballot_sync(0xffffffffu, sum + incl > at);
+      if (found) {
+        const int src = __ffs(found) - 1;
+        cb = b0 + src;
+        clen = __shfl_sync(0xffffffffu, n, src);
+        seq_begin = (sum + __shfl_sync(0xffffffffu, incl, src) - tiles_of(clen)) * hc;
+        break;
       }
-      if (!small_pages) {
-        const int id = __shfl_sync(0xffffffffu, my_id, (page - first_page) & 31);
-        if (lane == 0) {
-          const int r = pos - page * p.page_size;
-          const size_t so = ((size_t)id * p.Hkv + kvh) * groups + r / kGroup;
-          mbar_arrive_expect_tx(fb, S::kStageBytes + 32);
-          tma_load_4d(dst, &tmap_k, 0, r, kvh, id, fb, pol);
-          bulk_load(sc, p.k_scales + so, 16, fb);
-          tma_load_4d(dst + S::kTileBytes, &tmap_v, 0, r, kvh, id, fb, pol);
-          bulk_load(sc + 16, p.v_scales + so, 16, fb);
-        }
-      } else {
-        // pages of this tile that hold positions < len; later ones are not loaded
-        const int n = min(kTile / box, (len - pos + box - 1) / box);
-        if (lane == 0) mbar_arrive_expect_tx(fb, n * 2 * box * D);
-        __syncwarp();
-        // lane j < n: page j of the tile
-        const int id = __shfl_sync(0xffffffffu, my_id, (page - first_page + lane) & 31);
-        if (lane < n) {
-          tma_load_4d(dst + lane * box * D, &tmap_k, 0, 0, kvh, id, fb, pol);
-          tma_load_4d(dst + S::kTileBytes + lane * box * D, &tmap_v, 0, 0, kvh, id, fb, pol);
-        }
-        // lanes 0 .. 7: scale `lane & 3` of K (0 .. 3) or V (4 .. 7)
-        const int g = lane & 3, pg = g * kGroup / box;
-        const int gid = __shfl_sync(0xffffffffu, my_id, (page - first_page + pg) & 31);
-        if (lane < 8) {
-          if (pg < n) {
-            const size_t so = ((size_t)gid * p.Hkv + kvh) * groups + (g - pg * groups);
-            cp_async_4(sc + lane * 4, (lane < 4 ? p.k_scales : p.v_scales) + so);
-          }
-          cp_async_arrive_noinc(fb);
-        }
+      sum += __shfl_sync(0xffffffffu, incl, 31);
+      b0 += 32;
+      n = b0 + lane < p.B ? len_of(b0 + lane) : 0;
+    }
+  }
+
+  // ---- loads.  Lane (j, i) of a chunk of tiles has page i of the chunk's j-th tile: its
+  // id, the tile's position and row in the page, its segment in the sequence and its
+  // pages with positions < len (later ones are not loaded).
+  const int box = min(p.page_size, kTile);  // rows of a TMA box
+  const int box_bits = p.page_size >= 64 ? 6 : p.page_size >= 32 ? 5 : 4;
+  const int page_bits = kTileBits - box_bits;  // log2 of a tile's pages
+  const int chunk_bits = 5 - page_bits;     // log2 of a chunk's tiles
+  const int groups = p.page_size / kGroup;
+  const uint64_t pol = l2_policy_evict_first();
+  int lb = cb, lbegin = seq_begin, llen = clen;  // this lane's sequence
+  int id_next = 0, pos_next = 0, row_next = 0, seg_next = 0, n_next = 0;
+  auto load_chunk = [&](int c) {
+    const int j = (c << chunk_bits) + (lane >> page_bits);
+    id_next = 0;
+    if (j < nj) {
+      int n = tiles_of(llen), x = g0 + j - lbegin;
+      while (x >= n * hc) {
+        lbegin += n * hc;
+        x -= n * hc;
+        llen = len_of(++lb);
+        n = tiles_of(llen);
+      }
+      seg_next = div_estimated(x, n);
+      pos_next = (x - seg_next * n) * kTile;
+      const int page = p.by_page(pos_next), mine = lane & ((1 << page_bits) - 1);
+      row_next = pos_next - page * p.page_size;
+      n_next = page_bits == 0 ? 1 : min(1 << page_bits, (llen - pos_next + box - 1) >> box_bits);
+      if (mine < n_next) id_next = p.block_table[(size_t)lb * p.max_pages + page + mine];
+    }
+  };
+  int ids = 0, rows_in = 0, whats = 0, chunk = -1;
+  // The scales of the tiles in flight, oldest first: lanes 0 .. kBlocks - 1 have K's, the next kBlocks V's.
+  float scale_in[kRing];
+#pragma unroll
+  for (int i = 0; i < kRing; ++i) scale_in[i] = 0.f;
+  // The whole warp: start the loads of its j-th tile into slot j % kRing, and of its scales into `mine`.
+  auto issue = [&](int j, float& mine) {
+    if (j >= nj) return;
+    const bool fresh = (j >> chunk_bits) != chunk;
+    if (fresh) {
+      chunk = j >> chunk_bits;
+      ids = id_next;
+      rows_in = row_next;
+      whats = p.by_chunks(seg_next) << 3 | n_next;
+      if (ids < 0 || ids >= p.num_pages) {
+        set_status(p.status, kDevBadIndex);
+        ids = 0;
       }
     }
-    if (!ok && lane == 0) set_status(p.status, kDevWaitTimeout);
-    return;
-  }
+    const int slot = j % kRing;
+    const uint32_t fb = full_bar + 8 * slot, dst = ring + slot * S::kSlotBytes;
+    const int src = (j << page_bits) & 31;
+    const int blk = lane % kBlocks, pg = (blk * kGroup) >> box_bits;  // this lane's block and its page in the tile
+    const int what = __shfl_sync(0xffffffffu, whats, src), r = __shfl_sync(0xffffffffu, rows_in, src);
+    const int id = __shfl_sync(0xffffffffu, ids, (src + lane) & 31);
+    const int gid = __shfl_sync(0xffffffffu, ids, (src + pg) & 31);
+    const int n = what & 7, kvh = what >> 3;
+    if (page_bits == 0) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(fb, S::kSlotBytes);
+        tma_load_4d(dst, &tmap_k, 0, r, kvh, id, fb, pol);
+        tma_load_4d(dst + S::kTileBytes, &tmap_v, 0, r, kvh, id, fb, pol);
+      }
+    } else {
+      if (lane == 0) mbar_arrive_expect_tx(fb, n * 2 * box * D);
+      __syncwarp();
+      if (lane < n) {
+        tma_load_4d(dst + lane * box * D, &tmap_k, 0, r, kvh, id, fb, pol);
+        tma_load_4d(dst + S::kTileBytes + lane * box * D, &tmap_v, 0, r, kvh, id, fb, pol);
+      }
+    }
+    if (lane < 2 * kBlocks && pg < n)
+      mine = (lane < kBlocks ? p.k_scales : p.v_scales)[((size_t)gid * p.Hkv + kvh) * groups +
+                                                        (r / kGroup + blk - (pg << box_bits) / kGroup)];
+    if (fresh && ((chunk + 1) << chunk_bits) < nj) load_chunk(chunk + 1);  // looked at a chunk later
+  };
+  load_chunk(0);
 
-  // --------------------------------------------------------------- consumers
+  // ---- the current tile: tile ct of segment sl of sequence cb (clen positions)
+  int ct = __shfl_sync(0xffffffffu, pos_next, 0) / kTile, sl = __shfl_sync(0xffffffffu, seg_next, 0);
   const int g = lane >> 2, t = lane & 3;
   const int lm = lane >> 3, lr = lane & 7;  // ldmatrix: matrix and row that this lane addresses
-
   // Q as the column operand: lane (g, t) holds row g's dims D/4 * t .. of each
   // tile of 8 rows, in the order in which the K words lie
   uint32_t qb[NT][kSteps][2];
-  float rowf[NT][2];  // scores to log2 units, for rows 2t and 2t + 1 of the tile
-  int lim[NT][2];     // positions that they see
+  auto load_q = [&]() {  // as it is; turned to f16 when its first tile is there
+    const int kvh = p.by_chunks(sl), row0 = (sl - kvh * p.chunks) * kRowsPerCta;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int r = 8 * n + g;
-    uint32_t w[D / 8];
-    float amax = 0.f;
+    for (int n = 0; n < NT; ++n) {
+      const int r = row0 + 8 * n + g;
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + row_at(cb, kvh, r) + t * (D / 4));
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      if (r < rows) u = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + row_at(row0 + r) + t * (D / 4))[i];
-      w[4 * i] = u.x;
-      w[4 * i + 1] = u.y;
-      w[4 * i + 2] = u.z;
-      w[4 * i + 3] = u.w;
+      for (int i = 0; i < D / 32; ++i) {
+        const uint4 u = r < p.T * p.grp ? q[i] : make_uint4(0u, 0u, 0u, 0u);
+        qb[n][2 * i][0] = u.x;
+        qb[n][2 * i][1] = u.y;
+        qb[n][2 * i + 1][0] = u.z;
+        qb[n][2 * i + 1][1] = u.w;
+      }
     }
+  };
+  if (nj > 0) load_q();
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      const float2 f = unpack2<T>(w[i]);
-      amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-    }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    // 2^14 <= amax 2^(14 - e) < 2^15; zero and infinite rows stay as they are
-    int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-    e = amax > 0.f && amax < INFINITY ? max(e, -100) : 14;
-    const float up = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
-    const float down = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23);
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      const float2 f = unpack2<T>(w[i]);
-      qb[n][i >> 1][i & 1] = pack2<__half>(f.x * up, f.y * up);
-    }
-    // rows 2t, 2t + 1 belong to lanes with g = 2t, 2t + 1
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      rowf[n][j] = __shfl_sync(0xffffffffu, down, (2 * t + j) * 4) * p.scale_log2;
-      lim[n][j] = min(len, len - p.T + 1 + (row0 + 8 * n + 2 * t + j) / p.grp);
-    }
-  }
-  const int lim_min = len - p.T + 1 + row0 / p.grp;  // positions that every row sees
+  for (int j = 0; j < kRing; ++j) issue(j, scale_in[j]);
 
+  float rowf[NT][2];  // scores to log2 units, for rows 2t and 2t + 1 of a tile of 8
+  int lim[NT][2];     // positions that they see
+  int lim_min = 0;    // positions that every row sees
   float acc[kChunks][NT][4];
-#pragma unroll
-  for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-    for (int n = 0; n < NT; ++n) acc[c][n][0] = acc[c][n][1] = acc[c][n][2] = acc[c][n][3] = 0.f;
   float mrow[NT][2], lrow[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    mrow[n][0] = mrow[n][1] = -INFINITY;
-    lrow[n][0] = lrow[n][1] = 0.f;
-  }
-  float vref = kMinScale;  // R
+  int vexp = -126;         // log2 R
+  bool begins = true;      // a portion begins with this tile
   bool ok = true;
 
-  for (int i = warp; i < nt; i += kWarps) {
-    const int slot = i % kStages;
-    if (!mbar_wait_bounded(full_bar + 8 * slot, (i / kStages) & 1)) {
+  // The portion's state as a record
+  auto emit_record = [&](float* rec) {
+    const float r = exp2_int(vexp);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = 8 * n + 2 * t + i;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+          *reinterpret_cast<float2*>(rec + row * kRow + 16 * c + 2 * g) =
+              make_float2(acc[c][n][i] * (1.f / kWeightUp) * r, acc[c][n][2 + i] * (1.f / kWeightUp) * r);
+        if (g == 0) *reinterpret_cast<float2*>(rec + kRows * kRow + 2 * row) = make_float2(mrow[n][i], lrow[n][i]);
+      }
+  };
+
+#pragma unroll 1
+  for (int j = 0; j < nj; ++j) {
+    if (begins) {
+      begins = false;
+      const int row0 = (sl - p.by_chunks(sl) * p.chunks) * kRowsPerCta;
+      lim_min = clen - p.T + 1 + p.by_grp(row0);
+      vexp = -126;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        mrow[n][0] = mrow[n][1] = -INFINITY;
+        lrow[n][0] = lrow[n][1] = 0.f;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) acc[c][n][0] = acc[c][n][1] = acc[c][n][2] = acc[c][n][3] = 0.f;
+        float amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const float2 f = unpack2<T>(qb[n][i >> 1][i & 1]);
+          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        // 2^14 <= amax 2^(14 - e) < 2^15; zero and infinite rows stay as they are
+        int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+        e = amax > 0.f && amax < INFINITY ? max(e, -100) : 14;
+        const float up = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
+        const float down = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const float2 f = unpack2<T>(qb[n][i >> 1][i & 1]);
+          qb[n][i >> 1][i & 1] = pack2<__half>(f.x * up, f.y * up);
+        }
+        // rows 2t, 2t + 1 belong to lanes with g = 2t, 2t + 1
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          rowf[n][i] = __shfl_sync(0xffffffffu, down, (2 * t + i) * 4) * p.scale_log2;
+          lim[n][i] = min(clen, clen - p.T + 1 + p.by_grp(row0 + 8 * n + 2 * t + i));
+        }
+      }
+    }
+    const int slot = j % kRing;
+    if (!mbar_wait_bounded(full_bar + 8 * slot, (j / kRing) & 1)) {
       ok = false;
       break;
     }
-    const uint32_t kt = base + slot * S::kStageBytes, vt = kt + S::kTileBytes;
-    const float4 ks4 = ld_smem<float4>(sm, S::kScales + slot * 32);
-    float4 vs4 = ld_smem<float4>(sm, S::kScales + slot * 32 + 16);
-    const int pos0 = (t0 + i) * kTile;
+    const uint32_t kt = ring + slot * S::kSlotBytes, vt = kt + S::kTileBytes;
+    const int pos0 = ct * kTile;
     const bool edge = pos0 + kTile > lim_min;  // some row does not see all of the tile
-    if (pos0 + kTile > len) {
+    float ks[kBlocks], vs[kBlocks];
+#pragma unroll
+    for (int m = 0; m < kBlocks; ++m) {
+      ks[m] = __shfl_sync(0xffffffffu, scale_in[0], m);
+      vs[m] = __shfl_sync(0xffffffffu, scale_in[0], kBlocks + m);
+    }
+    if (pos0 + kTile > clen) {
       // V rows past the end may hold anything (NaN times p = 0 would still be NaN), and so may their blocks' scales
-      const int left = len - pos0;
+      const int left = clen - pos0;
       for (int e = left * (D / 16) + lane; e < kTile * (D / 16); e += 32)
         sts128(vt + S::at(e / (D / 16), e % (D / 16)), make_uint4(0u, 0u, 0u, 0u));
-      if (left <= 16) vs4.y = 0.f;
-      if (left <= 32) vs4.z = 0.f;
-      if (left <= 48) vs4.w = 0.f;
+#pragma unroll
+      for (int m = 1; m < kBlocks; ++m)
+        if (left <= kGroup * m) vs[m] = 0.f;
       __syncwarp();
     }
-    const float ks[4] = {ks4.x, ks4.y, ks4.z, ks4.w};
-    const float vs[4] = {vs4.x, vs4.y, vs4.z, vs4.w};
 
     // ---- S^T = K Q^T, 16 positions (one block of the cache) at a time
-    float s[4][NT][4];
+    float s[kBlocks][NT][4];
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
+    for (int m = 0; m < kBlocks; ++m) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.f;
 #pragma unroll
@@ -340,38 +529,36 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
     for (int n = 0; n < NT; ++n) {
       mt[n][0] = mt[n][1] = -INFINITY;
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+      for (int m = 0; m < kBlocks; ++m)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float x = s[m][n][j] * (ks[m] * rowf[n][j & 1]);
-          if (edge && pos0 + 16 * m + g + 8 * (j >> 1) >= lim[n][j & 1]) x = -INFINITY;
-          s[m][n][j] = x;
-          mt[n][j & 1] = fmaxf(mt[n][j & 1], x);
+        for (int i = 0; i < 4; ++i) {
+          float x = s[m][n][i] * (ks[m] * rowf[n][i & 1]);
+          if (edge && pos0 + 16 * m + g + 8 * (i >> 1) >= lim[n][i & 1]) x = -INFINITY;
+          s[m][n][i] = x;
+          mt[n][i & 1] = fmaxf(mt[n][i & 1], x);
         }
     }
     // ---- running maximum and V reference; rescale what was summed before
-    const float vtop = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-    float vgrow = 1.f;
-    if (vtop > vref) {
-      const uint32_t up = min((__float_as_uint(vtop) + 0x7FFFFFu) & 0x7F800000u, 0x7F000000u);  // next power of two
-      vgrow = vref / __uint_as_float(up);
-      vref = __uint_as_float(up);
-    }
-    const float vinv = 1.f / vref;
-    float mref[NT][2];
+    float vtop = vs[0];
+#pragma unroll
+    for (int m = 1; m < kBlocks; ++m) vtop = fmaxf(vtop, vs[m]);
+    const int vneed = min(static_cast<int>((__float_as_uint(vtop) + 0x7FFFFFu) >> 23) - 127, 126);
+    const float vgrow = exp2_int(min(vexp - vneed, 0));
+    vexp = max(vexp, vneed);
+    const float vinv = exp2_int(-vexp);
+    float mref[NT][2], alpha[NT][2];
     bool moved = vgrow != 1.f;
-    float alpha[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) mt[n][j] = fmaxf(mt[n][j], __shfl_xor_sync(0xffffffffu, mt[n][j], x));
-        const float mn = fmaxf(mrow[n][j], mt[n][j]);
-        mref[n][j] = mn == -INFINITY ? 0.f : mn;
-        moved |= mn != mrow[n][j];
-        alpha[n][j] = exp2_fast(mrow[n][j] - mref[n][j]);
-        mrow[n][j] = mn;
+        for (int x = 4; x < 32; x <<= 1) mt[n][i] = fmaxf(mt[n][i], __shfl_xor_sync(0xffffffffu, mt[n][i], x));
+        const float mn = fmaxf(mrow[n][i], mt[n][i]);
+        mref[n][i] = mn == -INFINITY ? 0.f : mn;
+        moved |= mn != mrow[n][i];
+        alpha[n][i] = exp2_fast(mrow[n][i] - mref[n][i]);
+        mrow[n][i] = mn;
       }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -390,7 +577,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
     }
     // ---- weights, and O^T += V^T P^T
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
+    for (int m = 0; m < kBlocks; ++m) {
       const float vm = vs[m] * vinv * kWeightUp;
       uint32_t pb[NT][2];
 #pragma unroll
@@ -419,117 +606,226 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
     }
     fence_proxy_async_smem();  // our reads and zeros of this slot precede its refill
     __syncwarp();
-    if (lane == 0) mbar_arrive(empty_bar + 8 * slot);
+#pragma unroll
+    for (int i = 0; i + 1 < kRing; ++i) scale_in[i] = scale_in[i + 1];
+    issue(j + kRing, scale_in[kRing - 1]);
+
+    // ---- the end of a portion
+    const int n_tiles = tiles_of(clen);
+    ++ct;
+    if (ct < n_tiles && j + 1 < nj) continue;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) lrow[n][i] += __shfl_xor_sync(0xffffffffu, lrow[n][i], x);
+    const int end = g0 + j + 1 - ct + n_tiles, begin = end - n_tiles;  // the segment in the flat order
+    const Portion mine = {cb * hc + sl, begin, end};
+    if (begin >= g0 && ct == n_tiles) {  // all of the segment
+      const float r = exp2_int(vexp);
+      const int kvh = p.by_chunks(sl), row0 = (sl - kvh * p.chunks) * kRowsPerCta;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = row0 + 8 * n + 2 * t + i;
+          if (row < p.T * p.grp) {
+            const float inv = (lrow[n][i] == 0.f ? 0.f : 1.0f / lrow[n][i]);
+            T* to = o + row_at(cb, kvh, row) + 2 * g;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+              *reinterpret_cast<uint32_t*>(to + 16 * c) =
+                  pack2<T>(acc[c][n][i] * (1.f / kWeightUp) * r * inv, acc[c][n][2 + i] * (1.f / kWeightUp) * r * inv);
+          }
+        }
+    } else if (j + 1 < nj) {  // the end of a segment that an earlier warp began
+      emit_record(p.first_rec + (size_t)(cta * kWarps + warp) * kRec);
+      if (lane == 0) portions[0] = mine;
+    } else {
+      emit_record(reinterpret_cast<float*>(sm + warp * S::kWarpBytes));  // over the drained ring
+      if (lane == 0) portions[1] = mine;
+    }
+    if (j + 1 < nj) {  // the next segment
+      begins = true;
+      ct = 0;
+      if (++sl == hc) {
+        sl = 0;
+        do clen = len_of(++cb);
+        while (clen == 0);
+      }
+      load_q();
+    }
   }
   if (!ok) set_status(p.status, kDevWaitTimeout);
 
-  // ---- the warps' states -> shared memory, over the ring once every warp is through
-  float* warp_o = reinterpret_cast<float*>(sm);
-  float* warp_ml = reinterpret_cast<float*>(sm + S::kMl);
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1) lrow[n][j] += __shfl_xor_sync(0xffffffffu, lrow[n][j], x);
-  named_barrier(1, kWarps * 32);
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int row = 8 * n + 2 * t + j;
-      float* wo = warp_o + (warp * kRowsPerCta + row) * D;
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c)
-        *reinterpret_cast<float2*>(wo + 16 * c + 2 * g) = make_float2(acc[c][n][j] * (1.f / kWeightUp) * vref, acc[c][n][2 + j] * (1.f / kWeightUp) * vref);
-      if (g == 0)
-        *reinterpret_cast<float2*>(warp_ml + (warp * kRowsPerCta + row) * 2) = make_float2(mrow[n][j], lrow[n][j]);
-    }
-  named_barrier(1, kWarps * 32);
-
-  // ---- merge the warps; a thread has one row's 4 dims
-  const int items = rows * (D / 4);
-  for (int e = threadIdx.x; e < items; e += kWarps * 32) {
-    const int row = e / (D / 4), d = (e - row * (D / 4)) * 4;
-    float mm = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, warp_ml[(w * kRowsPerCta + row) * 2]);
-    const float mu = mm == -INFINITY ? 0.f : mm;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float wgt = exp2_fast(warp_ml[(w * kRowsPerCta + row) * 2] - mu);
-      const float4 v = *reinterpret_cast<const float4*>(warp_o + (w * kRowsPerCta + row) * D + d);
-      a.x += wgt * v.x;
-      a.y += wgt * v.y;
-      a.z += wgt * v.z;
-      a.w += wgt * v.w;
-      l += wgt * warp_ml[(w * kRowsPerCta + row) * 2 + 1];
-    }
-    if (splits == 1) {
-      const float inv = l == 0.f ? 0.f : 1.0f / l;
-      store4(o + row_at(row0 + row) + d, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
-    } else {
-      const size_t rec = ((size_t)bhc * p.splits + split) * kRowsPerCta + row;
-      *reinterpret_cast<float4*>(p.part_o + rec * D + d) = a;
-      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + rec * 2) = make_float2(mm, l);
-    }
+  // ---- merge the portions of each segment; a thread has one row's 4 dims
+  Portion* parts = reinterpret_cast<Portion*>(sm + S::kParts);
+  int* last = reinterpret_cast<int*>(sm + S::kLast);
+  if (threadIdx.x < 2) {
+    parts[threadIdx.x].seg = -1;
+    last[threadIdx.x] = 0;
   }
-  if (splits == 1) return;
-
-  // ---- join of the splits by the last CTA of this (sequence, KV head, rows).  The
-  // barrier orders this CTA's partial stores before thread 0's acquire-release
-  // increment, which publishes them; in the last CTA the same increment and the
-  // barrier behind it order its loads.
-  int* last = reinterpret_cast<int*>(sm + S::kFlag);
-  named_barrier(1, kWarps * 32);
-  if (threadIdx.x == 0) *last = atom_add_acq_rel_gpu(p.counters + bhc, 1u) == (unsigned int)(splits - 1);
-  named_barrier(1, kWarps * 32);
-  if (!*last) return;
-  for (int e = threadIdx.x; e < items; e += kWarps * 32) {
-    const int row = e / (D / 4), d = (e - row * (D / 4)) * 4;
-    const size_t rec0 = (size_t)bhc * p.splits * kRowsPerCta + row;
-    float mu = -INFINITY, l = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s0 = 0; s0 < splits; s0 += kCombineBatch) {
-      float2 ml[kCombineBatch];
-      float4 v[kCombineBatch];
+  __syncthreads();
+  const Portion* all = reinterpret_cast<const Portion*>(sm + S::kPortions);
+  // lanes 2w and 2w + 1 look after warp w's first and last portion
+  const int seg_in = lane < 2 * kWarps ? all[lane].seg : -1;
+  unsigned int todo = __ballot_sync(0xffffffffu, seg_in >= 0);
+  int turn = threadIdx.x;  // segments start at different warps, so that they are merged side by side
+  while (todo) {
+    // a segment's portions here: the last ones of some warps, then perhaps the first one of the next warp
+    const Portion seg = all[__ffs(todo) - 1];
+    const unsigned int mask = __ballot_sync(0xffffffffu, seg_in == seg.seg);
+    todo &= ~mask;
+    const int b = p.by_hc(seg.seg), s2 = seg.seg - b * hc, kvh = p.by_chunks(s2);
+    const int row0 = (s2 - kvh * p.chunks) * kRowsPerCta, rows = min(kRowsPerCta, p.T * p.grp - row0);
+    const bool whole = seg.begin >= f0 && seg.end <= f1;
+    const int part = seg.begin < f0 ? 0 : 1;
+    if (!whole && threadIdx.x == 0) parts[part] = seg;
+    float* rec = p.cta_rec + (size_t)(2 * cta + part) * kRec;
+    const unsigned int firsts = mask & 0x55555555u;
+    const float* first = p.first_rec + (size_t)(cta * kWarps + (__ffs(firsts) >> 1)) * kRec;
+    const int items = rows * (D / 4);
+    for (int e = turn; e < items; e += kDecodeThreads) {
+      const int row = e / (D / 4), d = (e - row * (D / 4)) * 4;
+      float2 ml[kWarps + 1];
+      float4 v[kWarps + 1];
 #pragma unroll
-      for (int u = 0; u < kCombineBatch; ++u) {
-        ml[u] = make_float2(-INFINITY, 0.f);
-        v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (s0 + u < splits) {
-          const size_t rec = rec0 + (size_t)(s0 + u) * kRowsPerCta;
-          ml[u] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + rec * 2));
-          v[u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + rec * D + d));
+      for (int w = 0; w <= kWarps; ++w) {
+        ml[w] = make_float2(-INFINITY, 0.f);
+        v[w] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float* r = w < kWarps ? reinterpret_cast<const float*>(sm + w * S::kWarpBytes) : first;
+        if (w < kWarps ? (mask >> (2 * w + 1) & 1) != 0 : firsts != 0) {
+          ml[w] = *reinterpret_cast<const float2*>(r + kRows * kRow + 2 * row);
+          v[w] = *reinterpret_cast<const float4*>(r + row * kRow + d);
         }
       }
-      float nm = mu;
+      float mm = ml[0].x;
 #pragma unroll
-      for (int u = 0; u < kCombineBatch; ++u) nm = fmaxf(nm, ml[u].x);
-      const float ref = nm == -INFINITY ? 0.f : nm;
-      const float r = exp2_fast(mu - ref);
-      a.x *= r;
-      a.y *= r;
-      a.z *= r;
-      a.w *= r;
-      l *= r;
+      for (int w = 1; w <= kWarps; ++w) mm = fmaxf(mm, ml[w].x);
+      const float mu = mm == -INFINITY ? 0.f : mm;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l = 0.f;
 #pragma unroll
-      for (int u = 0; u < kCombineBatch; ++u) {
-        const float wgt = exp2_fast(ml[u].x - ref);
-        a.x += wgt * v[u].x;
-        a.y += wgt * v[u].y;
-        a.z += wgt * v[u].z;
-        a.w += wgt * v[u].w;
-        l += wgt * ml[u].y;
+      for (int w = 0; w <= kWarps; ++w) {
+        const float wgt = exp2_fast(ml[w].x - mu);
+        a.x += wgt * v[w].x;
+        a.y += wgt * v[w].y;
+        a.z += wgt * v[w].z;
+        a.w += wgt * v[w].w;
+        l += wgt * ml[w].y;
       }
-      mu = nm;
+      if (whole) {
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        store4(o + row_at(b, kvh, row0 + row) + d, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+      } else {
+        *reinterpret_cast<float4*>(rec + row * kRow + d) = a;
+        if (d == 0) *reinterpret_cast<float2*>(rec + kRows * kRow + 2 * row) = make_float2(mm, l);
+      }
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    store4(o + row_at(row0 + row) + d, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+    turn = (turn + kDecodeThreads - items % kDecodeThreads) % kDecodeThreads;
   }
-  if (threadIdx.x == 0) p.counters[bhc] = 0u;  // zero again for the next call
+
+  // ---- join segments that lie in several CTAs: the last of them to arrive.  The
+  // barrier orders this CTA's record stores before the acquire-release
+  // increment, which publishes them; in the last CTA the same increment and the
+  // barrier behind it order its loads.
+  __syncthreads();
+  if (threadIdx.x < 2 && parts[threadIdx.x].seg >= 0) {
+    const Portion seg = parts[threadIdx.x];
+    int c0;
+    const unsigned int others = ctas_of(seg, c0) - 1;
+    last[threadIdx.x] = atom_add_acq_rel_gpu(p.counters + seg.seg, 1u) == others;
+  }
+  __syncthreads();
+  for (int part = 0; part < 2; ++part) {
+    if (!last[part]) continue;
+    const Portion seg = parts[part];
+    const int b = p.by_hc(seg.seg), s2 = seg.seg - b * hc, kvh = p.by_chunks(s2);
+    const int row0 = (s2 - kvh * p.chunks) * kRowsPerCta, rows = min(kRowsPerCta, p.T * p.grp - row0);
+    int c0;
+    const int n = ctas_of(seg, c0);
+    // A warp takes a row and, of many records, every kJoin-th; a lane has kLane dims of it.
+    const int ways = n > kBatch ? kJoin : 1;
+    for (int task = part && last[0] ? (warp + kWarps - rows % kWarps) % kWarps : warp; task < rows * ways; task += kWarps) {
+      const int row = ways == 1 ? task : task / kJoin, way = ways == 1 ? 0 : task % kJoin;
+      float mu = -INFINITY, l = 0.f;
+      float a[kLane];
+#pragma unroll
+      for (int i = 0; i < kLane; ++i) a[i] = 0.f;
+      for (int s0 = way; s0 < n; s0 += kBatch * ways) {
+        float2 ml[kBatch];
+        float v[kBatch][kLane];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int at = s0 + u * ways;
+          ml[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+          for (int i = 0; i < kLane; ++i) v[u][i] = 0.f;
+          if (at < n) {  // the segment's first CTA has it as its last, the others as their first
+            const float* rec = p.cta_rec + (size_t)(2 * (c0 + at) + (at == 0)) * kRec;
+            ml[u] = __ldcg(reinterpret_cast<const float2*>(rec + kRows * kRow + 2 * row));
+            const LaneVec x = __ldcg(reinterpret_cast<const LaneVec*>(rec + row * kRow) + lane);
+            memcpy(v[u], &x, sizeof(x));
+          }
+        }
+        float nm = mu;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) nm = fmaxf(nm, ml[u].x);
+        const float ref = nm == -INFINITY ? 0.f : nm;
+        const float r = exp2_fast(mu - ref);
+        l *= r;
+#pragma unroll
+        for (int i = 0; i < kLane; ++i) a[i] *= r;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const float wgt = exp2_fast(ml[u].x - ref);
+          l += wgt * ml[u].y;
+#pragma unroll
+          for (int i = 0; i < kLane; ++i) a[i] += wgt * v[u][i];
+        }
+        mu = nm;
+      }
+      if (ways == 1) {
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < kLane; i += 2)
+          *reinterpret_cast<uint32_t*>(o + row_at(b, kvh, row0 + row) + lane * kLane + i) = pack2<T>(a[i] * inv, a[i + 1] * inv);
+      } else {  // over the rings, which have been read
+        float* rec = reinterpret_cast<float*>(sm) + (size_t)task * (D + 4);
+        LaneVec x;
+        memcpy(&x, a, sizeof(x));
+        reinterpret_cast<LaneVec*>(rec)[lane] = x;
+        if (lane == 0) *reinterpret_cast<float2*>(rec + D) = make_float2(mu, l);
+      }
+    }
+    if (ways > 1) {
+      __syncthreads();
+      for (int row = warp; row < rows; row += kWarps) {
+        const float* rec = reinterpret_cast<const float*>(sm) + (size_t)row * kJoin * (D + 4);
+        float mu = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int u = 0; u < kJoin; ++u) mu = fmaxf(mu, rec[u * (D + 4) + D]);
+        const float ref = mu == -INFINITY ? 0.f : mu;
+        float a[kLane];
+#pragma unroll
+        for (int i = 0; i < kLane; ++i) a[i] = 0.f;
+#pragma unroll
+        for (int u = 0; u < kJoin; ++u) {
+          const float wgt = exp2_fast(rec[u * (D + 4) + D] - ref);
+          l += wgt * rec[u * (D + 4) + D + 1];
+#pragma unroll
+          for (int i = 0; i < kLane; ++i) a[i] += wgt * rec[u * (D + 4) + lane * kLane + i];
+        }
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < kLane; i += 2)
+          *reinterpret_cast<uint32_t*>(o + row_at(b, kvh, row0 + row) + lane * kLane + i) = pack2<T>(a[i] * inv, a[i + 1] * inv);
+      }
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) p.counters[seg.seg] = 0u;  // zero again for the next call
+  }
 }
 
 // ---------------------------------------------------------------- host side
@@ -547,43 +843,34 @@ int check_decode(int B, int T, int Hq, int Hkv, int max_seq_len, int D) {
   return FOCAL_OK;
 }
 
-// One CTA per SM; a (sequence, KV head, rows) is split so that the CTAs fill the SMs once.
-void plan(int bhc, int max_seq_len, int sm_count, int* tiles_per_split, int* splits) {
-  const int tiles = (max_seq_len - 1) / kTile + 1;
-  const int s = std::max(1, std::min({sm_count / bhc, tiles, kMaxSplits}));
-  *tiles_per_split = (tiles + s - 1) / s;
-  *splits = (tiles + *tiles_per_split - 1) / *tiles_per_split;
-}
-
 size_t counter_bytes(int B, int T, int Hq, int Hkv) {
   const size_t n = (size_t)B * Hkv * row_chunks(T, Hq, Hkv) * 4;
   return (n + kCounterBytes - 1) / kCounterBytes * kCounterBytes;
 }
 
-// Splits of all (sequence, KV head, rows) together number at most the SMs, or
-// one each; 1024 covers any device's SMs.
+// Records: one per warp and two per CTA.
 size_t decode_workspace(int B, int T, int Hq, int Hkv, int max_seq_len, int D) {
-  const size_t bhc = (size_t)B * Hkv * row_chunks(T, Hq, Hkv);
   const size_t tiles = ((size_t)max_seq_len - 1) / kTile + 1;
-  const size_t smax = std::min({tiles, (size_t)kMaxSplits, std::max<size_t>(1, 1024 / bhc)});
-  const size_t recs = smax > 1 ? bhc * smax * kRowsPerCta : 0;
-  return counter_bytes(B, T, Hq, Hkv) + recs * (D + 2) * 4;
+  const size_t ctas = std::min<size_t>(kMaxCtas, tiles * B * Hkv * row_chunks(T, Hq, Hkv));
+  const size_t rows = T * (Hq / Hkv) <= 8 ? 8 : 16;
+  return counter_bytes(B, T, Hq, Hkv) + ctas * (warps_of(D) + 2) * rows * (D + 10) * 4;
 }
 
 int check_cache(const focal_kv8_cache* c);
 int check_cache_pointers(const focal_kv8_cache* c);
 
 template <typename T, int D, bool INT8, int NT>
-int launch_nt(const CUtensorMap& mk, const CUtensorMap& mv, const DecodeParams& p, dim3 grid, int slot,
+int launch_nt(const CUtensorMap& mk, const CUtensorMap& mv, const DecodeParams& p, int grid, int slot,
               cudaStream_t s) {
   auto kern = decode_kernel<T, D, INT8, NT>;
   const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), slot, Smem<D>::kBytes);
   if (rc) return rc;
-  return launch_pdl(kern, grid, kDecodeThreads, Smem<D>::kBytes, s, "kv8 decode_kernel launch", mk, mv, p);
+  return launch_pdl(kern, dim3(grid, 1, 1), 32 * warps_of(D), Smem<D>::kBytes, s, "kv8 decode_kernel launch", mk, mv,
+                    p);
 }
 
 template <typename T, int D>
-int launch_decode(const CUtensorMap& mk, const CUtensorMap& mv, const DecodeParams& p, int code, dim3 grid, int slot,
+int launch_decode(const CUtensorMap& mk, const CUtensorMap& mv, const DecodeParams& p, int code, int grid, int slot,
                   cudaStream_t s) {
   const bool one = p.T * p.grp <= 8;
   if (code == FOCAL_INT8)
@@ -640,8 +927,26 @@ int focal_kv8_decode(const void* q, void* o, const focal_kv8_cache* cache, const
   if (rc) return rc;
   DecodeParams p{};
   p.chunks = row_chunks(T, Hq, Hkv);
-  const int bhc = B * Hkv * p.chunks;
-  plan(bhc, max_seq_len, std::min(dev.sm_count, 1024), &p.tiles_per_split, &p.splits);
+  const int per_seg = (max_seq_len - 1) / kTile + 1;
+  const long long tiles = (long long)B * Hkv * p.chunks * per_seg;
+  if (tiles > INT32_MAX / 2) return set_error(FOCAL_ERR_UNSUPPORTED, "B * Hkv * max_seq_len too large");
+  const int sms = std::min(dev.sm_count, kMaxCtas);
+  p.segs = B * Hkv * p.chunks;
+  p.stack = (p.segs - 1) / sms + 1;
+  p.ways = sms / p.segs;
+  if (p.ways > 0) {
+    // One CTA where its warps have hardly more than a tile each, or else parts of 4 tiles or more; and not so many
+    // that joining them (110 cycles each) costs more than it saves (560 a tile).
+    const int most = (int)(2.25 * std::sqrt((double)per_seg)) + 1;
+    p.ways = per_seg <= warps_of(D) * 3 / 2 ? 1 : std::min({p.ways, (per_seg + 3) / 4, most});
+    p.per = (per_seg + p.ways - 1) / p.ways;
+    p.ways = (per_seg + p.per - 1) / p.per;
+    p.by_ways.set(p.ways);
+  }
+  // parts this small cannot be uneven enough to matter
+  p.decide = p.ways == 0 || p.per > warps_of(D) * 3 / 2;
+  const int ctas = p.decide ? (int)std::min<long long>(std::max<long long>((tiles + 3) / 4, (long long)p.segs * p.ways), sms)
+                            : p.segs * p.ways;
   p.q = q;
   p.o = o;
   p.k_scales = cache->k_scales;
@@ -650,9 +955,10 @@ int focal_kv8_decode(const void* q, void* o, const focal_kv8_cache* cache, const
   p.seq_lens = seq_lens;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.counters = reinterpret_cast<unsigned int*>(ws);
-  p.part_o = reinterpret_cast<float*>(ws + counter_bytes(B, T, Hq, Hkv));
-  p.part_ml = p.part_o + (size_t)bhc * p.splits * kRowsPerCta * D;
+  p.cta_rec = reinterpret_cast<float*>(ws + counter_bytes(B, T, Hq, Hkv));
+  p.first_rec = p.cta_rec + (size_t)ctas * 2 * (T * (Hq / Hkv) <= 8 ? 8 : 16) * (D + 10);
   p.status = dev.status;
+  p.B = B;
   p.T = T;
   p.Hq = Hq;
   p.Hkv = Hkv;
@@ -662,6 +968,11 @@ int focal_kv8_decode(const void* q, void* o, const focal_kv8_cache* cache, const
   p.max_pages = max_pages_per_seq;
   p.max_len = max_seq_len;
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.by_hc.set(Hkv * p.chunks);
+  p.by_chunks.set(p.chunks);
+  p.by_grp.set(p.grp);
+  p.by_page.set(cache->page_size);
+  p.by_grid.set(ctas);
 
   // pages [num_pages, Hkv, page_size, D] of bytes; boxes of min(page_size, 64) rows
   CUtensorMap mk, mv;
@@ -673,12 +984,11 @@ int focal_kv8_decode(const void* q, void* o, const focal_kv8_cache* cache, const
   if (rc) return rc;
   rc = encode_tensor_map(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, cache->v_pages, dims, strides, box, sw);
   if (rc) return rc;
-  const dim3 grid(p.splits, B * Hkv, p.chunks);
   if (dtype == FOCAL_BF16)
-    return D == 128 ? launch_decode<__nv_bfloat16, 128>(mk, mv, p, cache->code, grid, 44, stream)
-                    : launch_decode<__nv_bfloat16, 64>(mk, mv, p, cache->code, grid, 48, stream);
-  return D == 128 ? launch_decode<__half, 128>(mk, mv, p, cache->code, grid, 52, stream)
-                  : launch_decode<__half, 64>(mk, mv, p, cache->code, grid, 56, stream);
+    return D == 128 ? launch_decode<__nv_bfloat16, 128>(mk, mv, p, cache->code, ctas, 44, stream)
+                    : launch_decode<__nv_bfloat16, 64>(mk, mv, p, cache->code, ctas, 48, stream);
+  return D == 128 ? launch_decode<__half, 128>(mk, mv, p, cache->code, ctas, 52, stream)
+                  : launch_decode<__half, 64>(mk, mv, p, cache->code, ctas, 56, stream);
 }
 
 }  // extern "C"

@@ -370,13 +370,16 @@ def test_attention_nan_where_it_is_seen(cuda):
 
 
 def test_attention_is_deterministic_and_shares_pages(cuda):
-    """Two sequences over the same pages give the same bits, and so does every repetition."""
+    """Two sequences over the same pages agree within the bounds (where their tiles are split
+    between the SMs depends on their place in the batch), and every repetition gives the same bits."""
     table, pages = table_for([5000], 64, cuda, seed=8)
     cache = random_cache(pages, 8, 64, 128, E4M3, cuda, seed=8)
-    q = torch.randn(1, 32, 128, device=cuda, generator=gen(cuda, 9)).to(BF16).expand(2, 32, 128).contiguous()
-    args = (cache, table.expand(2, -1).contiguous(), ints([5000, 5000], cuda), 5000)
+    q = torch.randn(1, 1, 32, 128, device=cuda, generator=gen(cuda, 9)).to(BF16).expand(2, 1, 32, 128).contiguous()
+    table = table.expand(2, -1).contiguous()
+    args = (cache, table, ints([5000, 5000], cuda), 5000)
     first = F.gqa_decode_attention_kv8(q, *args)
-    assert torch.equal(first[0], first[1])
+    bounds = ok.attention(q, doubles(cache), table.cpu(), [5000, 5000])
+    assert torch.all((first.double() - bounds[0]).abs() <= attention_tolerance(bounds, BF16, 128))
     for _ in range(20):
         assert torch.equal(F.gqa_decode_attention_kv8(q, *args), first)
 

@@ -20,7 +20,7 @@ DeviceInfo g_info[kMaxDevices];
 std::once_flag g_info_once[kMaxDevices];
 int g_info_err[kMaxDevices];
 
-constexpr int kMaxKernelSlots = 64;
+constexpr int kMaxKernelSlots = 96;
 std::mutex g_smem_mutex;
 int g_smem_set[kMaxDevices][kMaxKernelSlots];
 

@@ -19,9 +19,16 @@
 // one more rounding when a block grows.
 //
 // One warp takes one (block, head) of K or of V, or 16 rows of one query head:
-// a lane holds 8 dims of every (32 / (D / 8))-th row in fp32 registers, so the
-// rows are read once and amax needs one warp reduction.  The cos and sin of the
-// block's rows are computed once per thread block into shared memory.
+// a lane holds 16 dims of every (32 / (D / 16))-th row in fp32 registers, so the
+// rows are read once and amax needs one warp reduction; the next job's rows are
+// on their way to shared memory meanwhile.  The cos and sin of the
+// block's rows are computed once per thread block into shared memory: of many
+// rows, eight follow from one angle by turning it on by inv_freq in 64 bits.
+//
+// Bound: HBM and the issue of about 600 instructions a job for prompts (8 x 1024
+// tokens of 32 + 16 heads 38.4 us, 0.73 of the measured copy rate), the chain of
+// dependent loads (length, then page and rows) for a step (8 tokens 4.1 us),
+// whose heads are spread over thread blocks.
 #include <algorithm>
 #include <cmath>
 
@@ -60,14 +67,41 @@ __device__ __forceinline__ uint32_t int8_code(float r) {
   return static_cast<uint32_t>(max(-127, min(127, c))) & 0xFFu;
 }
 
-// Four codes of x / scale; scale > 0.
+// Four codes of x / scale, the IEEE quotient rounded to the nearest even code;
+// scale > 0, inv = 1 / scale.
+//  e4m3: if scale is a power of two (`exact`), the product with inv is the quotient.
+//  int8: x * inv is within 1.6e-5 of the quotient (at most 127), so it rounds to
+//  the same integer unless it lies that near a half; then, and for infinities
+//  and NaN, the quotient itself is rounded.  Adding 1.5 2^23 leaves the nearest
+//  integer in the low bits.
 template <bool INT8>
-__device__ __forceinline__ uint32_t quantise4(const float* x, float scale) {
-  if (INT8)
+__device__ __forceinline__ uint32_t quantise4(const float* x, float scale, float inv, bool exact) {
+  if (INT8) {
+    constexpr float kRound = 12582912.f;
+    float t[4];
+    bool sure = true;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float q = __fmul_rn(x[e], inv);
+      t[e] = __fadd_rn(q, kRound);
+      sure = sure && fabsf(__fsub_rn(q, __fsub_rn(t[e], kRound))) <= 0.49998f;
+    }
+    if (sure) {
+      const uint32_t a = prmt(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040u);
+      const uint32_t b = prmt(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040u);
+      return prmt(a, b, 0x5410u);
+    }
     return int8_code(__fdiv_rn(x[0], scale)) | int8_code(__fdiv_rn(x[1], scale)) << 8 |
            int8_code(__fdiv_rn(x[2], scale)) << 16 | int8_code(__fdiv_rn(x[3], scale)) << 24;
-  return f32x2_to_e4m3x2(__fdiv_rn(x[0], scale), __fdiv_rn(x[1], scale)) |
-         static_cast<uint32_t>(f32x2_to_e4m3x2(__fdiv_rn(x[2], scale), __fdiv_rn(x[3], scale))) << 16;
+  }
+  float q[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) q[e] = __fmul_rn(x[e], inv);
+  if (!exact) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = __fdiv_rn(x[e], scale);
+  }
+  return f32x2_to_e4m3x2(q[0], q[1]) | static_cast<uint32_t>(f32x2_to_e4m3x2(q[2], q[3])) << 16;
 }
 
 template <bool INT8>
@@ -85,11 +119,15 @@ __device__ __forceinline__ void dequantise4(uint32_t c, float (&x)[4]) {
 }
 
 template <typename T, int D, bool INT8, bool INTERLEAVED>
-__global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(const AppendParams p) {
-  constexpr int kLanes = D / 8;           // lanes of one row
-  constexpr int kRows = 32 / kLanes;      // rows that a warp holds side by side
+__global__ void __launch_bounds__(32 * kAppendWarps, 2) append_kernel(const AppendParams p) {
+  constexpr int kLanes = D / 16;      // lanes of one row
+  constexpr int kRows = 32 / kLanes;  // rows that a warp holds side by side
   constexpr int kPasses = kGroup / kRows;
-  __shared__ float2 cs[kGroup][D / 2];
+  constexpr int kJobBytes = kGroup * D * 2;  // 16 rows of a head
+  extern __shared__ __align__(16) uint8_t sm[];
+  // cos and sin of row r and frequency f: a lane reads 8 frequencies, two at a time, side by side with its neighbours
+  float2* cs = reinterpret_cast<float2*>(sm);
+  auto cs_at = [&](int r, int f) { return r * (D / 2) + ((f & 7) >> 1) * (p.half >> 2) + (f >> 3) * 2 + (f & 1); };
   griddep_launch_dependents();
   griddep_wait();
 
@@ -108,117 +146,172 @@ __global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(const AppendP
   const int at = static_cast<int>(at0);  // position of the block's row 0
   const int r0 = max(start - at, 0), r1 = min(len - at, kGroup);  // the new rows of the block
   const int page = p.block_table[(long long)b * p.max_pages + at / p.page_size];
+  const int tok = c0 + at - start;  // token of row r: tok + r
+
+  // ---- rows of this warp's next job into its half of a double buffer
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int jobs = 2 * p.Hkv + p.Hq;
+  const int j0 = blockIdx.y * p.jobs_per_block + warp, j1 = min(jobs, static_cast<int>(blockIdx.y + 1) * p.jobs_per_block);
+  uint8_t* mine = sm + kGroup * (D / 2) * 8 + warp * 2 * kJobBytes;
+  auto fetch = [&](int j, int slot) {
+    if (j < j1) {
+      const bool is_q = j >= 2 * p.Hkv, is_v = !is_q && j >= p.Hkv;
+      const int h = is_q ? j - 2 * p.Hkv : is_v ? j - p.Hkv : j;
+      const long long ts = is_q ? p.qt : is_v ? p.vt : p.kt, hs = is_q ? p.qh : is_v ? p.vh : p.kh;
+      const T* x = static_cast<const T*>(is_q ? p.q : is_v ? p.v : p.k) + h * hs + (long long)tok * ts;
+      constexpr int kChunks = D / 8;  // of 16 bytes in a row
+      const uint32_t to = smem_u32(mine + slot * kJobBytes) + lane % kChunks * 16;
+      x += lane % kChunks * 8;
+#pragma unroll
+      for (int i = 0; i < kGroup * kChunks / 32; ++i) {
+        const int r = lane / kChunks + i * (32 / kChunks);
+        if (r >= r0 && r < r1) cp_async_16(to + r * D * 2, x + (long long)r * ts);
+      }
+    }
+    cp_async_commit();
+  };
+  fetch(j0, 0);
+
+  // ---- cos and sin of the block's rows
+  if (r1 - r0 <= 4) {
+    for (int i = threadIdx.x; i < (r1 - r0) * p.half; i += 32 * kAppendWarps) {
+      const int r = i / p.half, f = i - r * p.half;
+      cs[cs_at(r0 + r, f)] = rope_cos_sin(static_cast<double>(at + r0 + r), p.inv_freq[f], p.mscale);
+    }
+  } else {
+    for (int i = threadIdx.x; i < 2 * p.half; i += 32 * kAppendWarps) {
+      const int h = i >= p.half ? 8 : 0, f = h ? i - p.half : i;
+      const double w = p.inv_freq[f];
+      double s, c, ds, dc;
+      cos_sin(static_cast<double>(at + h) * w, c, s);
+      cos_sin(w, dc, ds);
+      s *= p.mscale;
+      c *= p.mscale;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        cs[cs_at(h + r, f)] = make_float2(static_cast<float>(c), static_cast<float>(s));
+        const double x = c * dc - s * ds;
+        s = s * dc + c * ds;
+        c = x;
+      }
+    }
+  }
   if (page < 0 || page >= p.num_pages) {
     if (threadIdx.x == 0) set_status(p.status, kDevBadIndex);
     return;
   }
-  const int tok = c0 + at - start;  // token of row r: tok + r
-  for (int i = threadIdx.x; i < (r1 - r0) * p.half; i += 32 * kAppendWarps) {
-    const int r = i / p.half, f = i - r * p.half;
-    cs[r0 + r][f] = rope_cos_sin(static_cast<double>(at + r0 + r), p.inv_freq[f], p.mscale);
-  }
   __syncthreads();
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c = lane % kLanes, rr = lane / kLanes;
   const int rot = 2 * p.half;
-  // this lane's dims: d0 .. d0 + 3 and d1 .. d1 + 3; with `turns`, four pairs of frequencies 4c .. 4c + 3
-  const bool turns = INTERLEAVED ? 8 * c < rot : 4 * c < p.half;
-  int d0, d1;
-  if (INTERLEAVED) {
-    d0 = 8 * c;
-    d1 = d0 + 4;
-  } else {
-    d0 = turns ? 4 * c : 8 * c;
-    d1 = turns ? p.half + 4 * c : d0 + 4;
-  }
+  // this lane's dims: d0 .. d0 + 7 and d1 .. d1 + 7; with `turns`, pairs of frequencies 8c .. 8c + 7
+  const bool turns = 16 * c < rot;
+  const int d0 = !INTERLEAVED && turns ? 8 * c : 16 * c;
+  const int d1 = !INTERLEAVED && turns ? p.half + 8 * c : d0 + 8;
   const int sub = at % p.page_size;  // row of the page
-  const int jobs = 2 * p.Hkv + p.Hq;
-  const int j1 = min(jobs, static_cast<int>(blockIdx.y + 1) * p.jobs_per_block);
-  for (int j = blockIdx.y * p.jobs_per_block + warp; j < j1; j += kAppendWarps) {
+  int slot = 0;
+  for (int j = j0; j < j1; j += kAppendWarps, slot ^= 1) {
     const bool is_q = j >= 2 * p.Hkv, is_v = !is_q && j >= p.Hkv;
     const int h = is_q ? j - 2 * p.Hkv : is_v ? j - p.Hkv : j;
-    const long long ts = is_q ? p.qt : is_v ? p.vt : p.kt, hs = is_q ? p.qh : is_v ? p.vh : p.kh;
-    const T* x = static_cast<const T*>(is_q ? p.q : is_v ? p.v : p.k) + h * hs;
-    float val[kPasses][8];
+    fetch(j + kAppendWarps, slot ^ 1);
+    const long long ph = (long long)page * p.Hkv + h;
+    float* sp = (is_v ? p.v_scales : p.k_scales) + ph * (p.page_size / kGroup) + sub / kGroup;
+    const float old = !is_q && r0 > 0 ? *sp : 0.f;
+    // rows i * kRows .. of pass i: warps skip the passes without new rows
+    auto has = [&](int i) { return (i + 1) * kRows > r0 && i * kRows < r1; };
+    cp_async_wait<1>();
+    __syncwarp();
+    const uint8_t* x = mine + slot * kJobBytes + rr * D * 2;
+    float val[kPasses][16];
     float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-      const int r = i * kRows + rr;
-      uint2 u = make_uint2(0u, 0u), w = make_uint2(0u, 0u);
-      if (r >= r0 && r < r1) {
-        const T* row = x + (long long)(tok + r) * ts;
-        u = *reinterpret_cast<const uint2*>(row + d0);
-        w = *reinterpret_cast<const uint2*>(row + d1);
+      if (!has(i)) continue;
+      const uint4 u = *reinterpret_cast<const uint4*>(x + i * kRows * D * 2 + d0 * 2);
+      const uint4 w = *reinterpret_cast<const uint4*>(x + i * kRows * D * 2 + d1 * 2);
+      const uint32_t raw[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float2 f = unpack2<T>(raw[e]);
+        val[i][2 * e] = f.x;
+        val[i][2 * e + 1] = f.y;
       }
-      const float2 f0 = unpack2<T>(u.x), f1 = unpack2<T>(u.y), f2 = unpack2<T>(w.x), f3 = unpack2<T>(w.y);
-      val[i][0] = f0.x; val[i][1] = f0.y; val[i][2] = f1.x; val[i][3] = f1.y;
-      val[i][4] = f2.x; val[i][5] = f2.y; val[i][6] = f3.x; val[i][7] = f3.y;
-    }
-    if (!is_v && turns) {
+      if (!is_v && turns) {  // (rows of the pass that are not new hold anything, and are not used)
 #pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        const int r = i * kRows + rr;
-        if (r >= r0 && r < r1) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            rope_turn(INTERLEAVED ? val[i][2 * e] : val[i][e], INTERLEAVED ? val[i][2 * e + 1] : val[i][4 + e],
-                      cs[r][4 * c + e]);
+        for (int e = 0; e < 8; e += 2) {
+          const float4 a = *reinterpret_cast<const float4*>(cs + cs_at(i * kRows + rr, 8 * c + e));
+          rope_turn(INTERLEAVED ? val[i][2 * e] : val[i][e], INTERLEAVED ? val[i][2 * e + 1] : val[i][8 + e],
+                    make_float2(a.x, a.y));
+          rope_turn(INTERLEAVED ? val[i][2 * e + 2] : val[i][e + 1], INTERLEAVED ? val[i][2 * e + 3] : val[i][9 + e],
+                    make_float2(a.z, a.w));
         }
       }
     }
     if (is_q) {
-      T* y = static_cast<T*>(p.q_out) + (long long)h * D;
+      T* y = static_cast<T*>(p.q_out) + ((long long)(tok + rr) * p.Hq + h) * D;
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
         const int r = i * kRows + rr;
         if (r >= r0 && r < r1) {
-          T* row = y + (long long)(tok + r) * p.Hq * D;
-          *reinterpret_cast<uint2*>(row + d0) = make_uint2(pack2<T>(val[i][0], val[i][1]), pack2<T>(val[i][2], val[i][3]));
-          *reinterpret_cast<uint2*>(row + d1) = make_uint2(pack2<T>(val[i][4], val[i][5]), pack2<T>(val[i][6], val[i][7]));
+          T* row = y + (long long)i * kRows * p.Hq * D;
+          uint32_t w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = pack2<T>(val[i][2 * e], val[i][2 * e + 1]);
+          *reinterpret_cast<uint4*>(row + d0) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(row + d1) = make_uint4(w[4], w[5], w[6], w[7]);
         }
       }
+      __syncwarp();  // the buffer is read: the next job's fetch may fill it
       continue;
     }
     // infinities saturate and NaN is stored as NaN (e4m3) or 0 (int8); neither sets the scale
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i)
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = i * kRows + rr;
+      if (has(i) && r >= r0 && r < r1) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float m = fabsf(val[i][e]);
-        if (m < INFINITY) amax = fmaxf(amax, m);
+        for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(val[i][e]));  // not NaN
       }
+    }
+    if (__any_sync(0xffffffffu, amax == INFINITY)) {
+      amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = i * kRows + rr;
+        if (r >= r0 && r < r1) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (fabsf(val[i][e]) < INFINITY) amax = fmaxf(amax, fabsf(val[i][e]));
+        }
+      }
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    uint8_t* pages = is_v ? p.v_pages : p.k_pages;
-    float* scales = is_v ? p.v_scales : p.k_scales;
-    const long long ph = (long long)page * p.Hkv + h;
-    uint8_t* out = pages + (ph * p.page_size + sub) * D;
-    float* sp = scales + ph * (p.page_size / kGroup) + sub / kGroup;
-    const float old = r0 > 0 ? *sp : 0.f;
+    uint8_t* out = (is_v ? p.v_pages : p.k_pages) + (ph * p.page_size + sub) * D;
     const float scale = fmaxf(old, needed_scale<INT8>(amax));
+    const float inv = scale > 0.f ? 1.f / scale : 0.f;
+    const bool exact = (__float_as_uint(scale) & 0x7FFFFFu) == 0;
     if (r0 > 0 && scale > old) {
-      for (int r = rr; r < r0; r += kRows) {
-        uint32_t* a0 = reinterpret_cast<uint32_t*>(out + r * D + d0);
-        uint32_t* a1 = reinterpret_cast<uint32_t*>(out + r * D + d1);
-        float f[4], g[4];
-        dequantise4<INT8>(*a0, f);
-        dequantise4<INT8>(*a1, g);
+      for (int i = lane; i < r0 * (D / 4); i += 32) {  // four codes at a time
+        uint32_t* a = reinterpret_cast<uint32_t*>(out) + i;
+        float f[4];
+        dequantise4<INT8>(*a, f);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          f[e] *= old;
-          g[e] *= old;
-        }
-        *a0 = quantise4<INT8>(f, scale);
-        *a1 = quantise4<INT8>(g, scale);
+        for (int e = 0; e < 4; ++e) f[e] *= old;
+        *a = quantise4<INT8>(f, scale, inv, exact);
       }
     }
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       const int r = i * kRows + rr;
-      if (r >= r0 && r < r1) {
-        *reinterpret_cast<uint32_t*>(out + r * D + d0) = scale > 0.f ? quantise4<INT8>(val[i], scale) : 0u;
-        *reinterpret_cast<uint32_t*>(out + r * D + d1) = scale > 0.f ? quantise4<INT8>(val[i] + 4, scale) : 0u;
+      if (has(i) && r >= r0 && r < r1) {
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+        if (scale > 0.f) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = quantise4<INT8>(val[i] + 4 * e, scale, inv, exact);
+        }
+        *reinterpret_cast<uint2*>(out + r * D + d0) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(out + r * D + d1) = make_uint2(w[2], w[3]);
       }
     }
     __syncwarp();
@@ -247,15 +340,21 @@ int check_cache_pointers(const focal_kv8_cache* c) {
   return FOCAL_OK;
 }
 
+template <typename T, int D, bool INT8, bool INTERLEAVED>
+int launch_one(const AppendParams& p, int slot, dim3 grid, cudaStream_t s) {
+  constexpr int kBytes = kGroup * (D / 2) * 8 + kAppendWarps * 2 * kGroup * D * 2;  // cos and sin, double buffers
+  auto kern = append_kernel<T, D, INT8, INTERLEAVED>;
+  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), slot, kBytes);
+  if (rc) return rc;
+  return launch_pdl(kern, grid, 32 * kAppendWarps, kBytes, s, "append_kernel launch", p);
+}
+
 template <typename T, int D>
-int launch_append(const AppendParams& p, int code, bool interleaved, dim3 grid, cudaStream_t s) {
-  const char* what = "append_kernel launch";
-  const int n = 32 * kAppendWarps;
+int launch_append(const AppendParams& p, int code, bool interleaved, int slot, dim3 grid, cudaStream_t s) {
   if (code == FOCAL_INT8)
-    return interleaved ? launch_pdl(append_kernel<T, D, true, true>, grid, n, 0, s, what, p)
-                       : launch_pdl(append_kernel<T, D, true, false>, grid, n, 0, s, what, p);
-  return interleaved ? launch_pdl(append_kernel<T, D, false, true>, grid, n, 0, s, what, p)
-                     : launch_pdl(append_kernel<T, D, false, false>, grid, n, 0, s, what, p);
+    return interleaved ? launch_one<T, D, true, true>(p, slot, grid, s) : launch_one<T, D, true, false>(p, slot + 1, grid, s);
+  return interleaved ? launch_one<T, D, false, true>(p, slot + 2, grid, s)
+                     : launch_one<T, D, false, false>(p, slot + 3, grid, s);
 }
 
 }  // namespace kv8
@@ -326,13 +425,18 @@ extern "C" int focal_kv8_append(const focal_kv8_append_args* a, const focal_kv8_
   p.max_pages = a->max_pages_per_seq;
   p.pieces = static_cast<int>(pieces);
   p.mscale = a->mscale;
+  // Heads of a block of tokens are spread over thread blocks until these are
+  // three to an SM (every one of them computes cos and sin anew).
   const int jobs = 2 * Hkv + a->Hq;
-  p.jobs_per_block = jobs;
-  const dim3 grid(static_cast<unsigned>(pieces * a->B), 1, 1);
+  const long long blocks = std::min<long long>(pieces * a->B, (long long)a->T / kGroup + a->B);
+  const int spread = (int)std::min<long long>((jobs + kAppendWarps - 1) / kAppendWarps,
+                                              std::max<long long>(1, (3LL * dev.sm_count + blocks - 1) / blocks));
+  p.jobs_per_block = ((jobs + spread - 1) / spread + kAppendWarps - 1) / kAppendWarps * kAppendWarps;
+  const dim3 grid(static_cast<unsigned>(pieces * a->B), (jobs + p.jobs_per_block - 1) / p.jobs_per_block, 1);
   const bool il = a->interleaved != 0;
   if (a->dtype == FOCAL_BF16)
-    return D == 128 ? launch_append<__nv_bfloat16, 128>(p, cache->code, il, grid, stream)
-                    : launch_append<__nv_bfloat16, 64>(p, cache->code, il, grid, stream);
-  return D == 128 ? launch_append<__half, 128>(p, cache->code, il, grid, stream)
-                  : launch_append<__half, 64>(p, cache->code, il, grid, stream);
+    return D == 128 ? launch_append<__nv_bfloat16, 128>(p, cache->code, il, 60, grid, stream)
+                    : launch_append<__nv_bfloat16, 64>(p, cache->code, il, 64, grid, stream);
+  return D == 128 ? launch_append<__half, 128>(p, cache->code, il, 68, grid, stream)
+                  : launch_append<__half, 64>(p, cache->code, il, 72, grid, stream);
 }

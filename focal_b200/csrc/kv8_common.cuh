@@ -13,6 +13,19 @@ namespace kv8 {
 constexpr int kGroup = 16;  // consecutive tokens of a page and KV head that share a scale
 constexpr float kMinScale = 1.17549435e-38f;  // 2^-126: scales stay normal numbers
 
+// n / d for 0 <= n < 2^31 by a product and a shift (Granlund and Montgomery, 1994).
+struct FastDiv {
+  uint32_t mul, shift;
+  void set(uint32_t d) {
+    shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
+  }
+};
+
 // Two e4m3 codes (low byte first) as f16x2; every e4m3 value is exact in f16.
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t c) {
   uint32_t r;
@@ -50,12 +63,42 @@ __device__ __forceinline__ uint16_t f32x2_to_e4m3x2(float lo, float hi) {
   return r;
 }
 
+// cos and sin of a 64-bit angle, |a| < 2^50: less the nearest multiple of pi / 2,
+// which is subtracted in two parts (Cody and Waite), their Taylor series to
+// x^14 and x^13, off by less than 2^-45.  (CUDA's sincos is more exact and for any
+// angle, and took seven times as long; the result is rounded to fp32.)
+__device__ __forceinline__ void cos_sin(double a, double& c, double& s) {
+  constexpr double kShift = 6755399441055744.0;  // 1.5 2^52: the sum's low bits are the rounded integer
+  const double t = fma(a, 0.63661977236758134308, kShift);
+  const int quarter = __double2loint(t);
+  const double q = t - kShift;
+  const double r = fma(-q, 6.12323399573676603587e-17, fma(-q, 1.57079632679489661923, a));
+  const double x = r * r;
+  double u = 1.0 / 6227020800.0, v = -1.0 / 87178291200.0;
+  u = fma(u, x, -1.0 / 39916800.0);
+  v = fma(v, x, 1.0 / 479001600.0);
+  u = fma(u, x, 1.0 / 362880.0);
+  v = fma(v, x, -1.0 / 3628800.0);
+  u = fma(u, x, -1.0 / 5040.0);
+  v = fma(v, x, 1.0 / 40320.0);
+  u = fma(u, x, 1.0 / 120.0);
+  v = fma(v, x, -1.0 / 720.0);
+  u = fma(u, x, -1.0 / 6.0);
+  v = fma(v, x, 1.0 / 24.0);
+  v = fma(v, x, -0.5);
+  const double sr = fma(r * x, u, r), cr = fma(x, v, 1.0);
+  s = quarter & 1 ? cr : sr;
+  c = quarter & 1 ? sr : cr;
+  s = quarter & 2 ? -s : s;
+  c = (quarter + 1) & 2 ? -c : c;
+}
+
 // cos and sin of position * inv_freq, times mscale, each rounded once to fp32.
 // The angle and its reduction are 64-bit: at position 2^20 an fp32 angle is
 // off by up to 2^-5 radians, a 64-bit one by 2^-34.
 __device__ __forceinline__ float2 rope_cos_sin(double position, double inv_freq, double mscale) {
   double s, c;
-  sincos(__dmul_rn(position, inv_freq), &s, &c);
+  cos_sin(__dmul_rn(position, inv_freq), c, s);
   return make_float2(static_cast<float>(__dmul_rn(c, mscale)), static_cast<float>(__dmul_rn(s, mscale)));
 }
 

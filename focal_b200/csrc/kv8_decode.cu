@@ -60,19 +60,6 @@ constexpr int kBatch = 16;  // records whose loads a join has in flight
 constexpr int kJoin = 4;    // ways that many records are shared out
 constexpr float kWeightUp = 32768.f;
 
-// n / d for 0 <= n < 2^31 by a product and a shift (Granlund and Montgomery, 1994).
-struct FastDiv {
-  uint32_t mul, shift;
-  void set(uint32_t d) {
-    shift = 0;
-    while ((1ull << shift) < d) ++shift;
-    mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-  }
-  __device__ __forceinline__ int operator()(int n) const {
-    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
-  }
-};
-
 struct DecodeParams {
   const void* q;
   void* o;

@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 2) append_kernel(const Appe
   }
   if (page < 0 || page >= p.num_pages) {
     if (threadIdx.x == 0) set_status(p.status, kDevBadIndex);
+    cp_async_wait<0>();
     return;
   }
   __syncthreads();

@@ -50,8 +50,10 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
     hi = *reinterpret_cast<const uint32_t*>(&y);
   } else {
     if (STRIDED) w = prmt(w, 0u, 0x3120u);
-    lo = e4m3x2_to_f16x2(static_cast<uint16_t>(w));
-    hi = e4m3x2_to_f16x2(static_cast<uint16_t>(w >> 16));
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
   }
 }
 

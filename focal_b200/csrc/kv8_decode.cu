@@ -511,20 +511,30 @@ __global__ void __launch_bounds__(32 * warps_of(D))
       }
     }
     // ---- scale, mask, tile maximum
-    float mt[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      mt[n][0] = mt[n][1] = -INFINITY;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int m = 0; m < kBlocks; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = s[m][n][i] * (ks[m] * rowf[n][i & 1]);
-          if (edge && pos0 + 16 * m + g + 8 * (i >> 1) >= lim[n][i & 1]) x = -INFINITY;
-          s[m][n][i] = x;
-          mt[n][i & 1] = fmaxf(mt[n][i & 1], x);
-        }
+        for (int i = 0; i < 4; ++i) s[m][n][i] *= ks[m] * rowf[n][i & 1];
+    if (edge) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int m = 0; m < kBlocks; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (pos0 + 16 * m + g + 8 * (i >> 1) >= lim[n][i & 1]) s[m][n][i] = -INFINITY;
     }
+    float mt[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mt[n][i] = fmaxf(s[0][n][i], s[0][n][i + 2]);
+#pragma unroll
+        for (int m = 1; m < kBlocks; ++m) mt[n][i] = fmaxf(mt[n][i], fmaxf(s[m][n][i], s[m][n][i + 2]));
+      }
     // ---- running maximum and V reference; rescale what was summed before
     float vtop = vs[0];
 #pragma unroll

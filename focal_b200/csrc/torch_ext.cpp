@@ -9,6 +9,7 @@
 // All arithmetic happens in libfocal_b200.so behind include/focal_b200.h.
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -377,6 +378,11 @@ void check_rows(const torch::Tensor& t, const char* name, const torch::Tensor& l
   TORCH_CHECK(t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX && t.size(2) <= INT32_MAX, "unsupported size");
 }
 
+// torch::empty without the dispatcher, which costs more than such a step's kernel.
+torch::Tensor empty_like_rows(const torch::Tensor& t) {
+  return at::detail::empty_cuda(t.sizes(), t.scalar_type(), t.device(), c10::nullopt);
+}
+
 // A dimension of one element has no stride to speak of.
 int64_t stride_of(const torch::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 
@@ -412,7 +418,7 @@ torch::Tensor rope(torch::Tensor x, torch::Tensor positions, torch::Tensor inv_f
       at::assert_no_partial_overlap(y, x);
     }
   } else {
-    y = torch::empty(x.sizes(), x.options());
+    y = empty_like_rows(x);
   }
   raise_on(focal_rope(x.data_ptr(), y.data_ptr(), positions.data_ptr(), inv_freq.data_ptr<double>(), (int)x.size(0),
                       (int)x.size(1), (int)x.size(2), 2 * (int)inv_freq.size(0), interleaved, mscale, dtype,
@@ -496,7 +502,7 @@ c10::optional<torch::Tensor> kv8_append(torch::Tensor k, torch::Tensor v, torch:
     check_rows(*q, "q", k);
     TORCH_CHECK(inv_freq.has_value(), "q needs inv_freq: it is only turned");
     TORCH_CHECK(q->size(0) == T && q->size(2) == k.size(2), "q must have shape [T, Hq, D]");
-    turned = torch::empty(q->sizes(), q->options());
+    turned = empty_like_rows(*q);
     a.q = q->data_ptr();
     a.q_out = turned->data_ptr();
     a.Hq = (int)q->size(1);
@@ -536,7 +542,7 @@ torch::Tensor gqa_decode_attention_kv8(torch::Tensor q, torch::Tensor k_pages, t
   TORCH_CHECK(T <= INT32_MAX && Hq <= INT32_MAX && max_seq_len <= INT32_MAX && max_seq_len >= 1, "unsupported size");
   const double sc = scale.has_value() ? *scale : 1.0 / std::sqrt((double)D);
   const c10::cuda::CUDAGuard guard(q.device());
-  auto o = torch::empty(q.sizes(), q.options());
+  auto o = empty_like_rows(q);
   const cudaStream_t stream = current_stream();
   const size_t bytes =
       focal_kv8_decode_workspace_size((int)B, (int)T, (int)Hq, cache.num_kv_heads, (int)max_seq_len, (int)D);

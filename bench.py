@@ -970,7 +970,9 @@ def write_traffic_json(specs):
 def run_profile_case(args):
     """A few calls of one shape, for ncu captures of a single kernel:
     --profile-shape M,K,N (W4A16), --profile-attn B,L (attention) or
-    --profile-paged B,L,page_size (paged attention, pages shuffled)."""
+    --profile-paged B,L,page_size (paged attention, pages shuffled) or
+    --profile-kv8 B,L,page_size (a decode step's rotary positions, 8-bit append
+    and attention, behind L - 1 tokens of e4m3 codes)."""
     import torch
 
     import focal_b200 as F
@@ -994,6 +996,20 @@ def run_profile_case(args):
         table = torch.randperm(B * per, generator=g).to(torch.int32).view(B, per).to(dev)
         lens = torch.full((B,), L, dtype=torch.int32, device=dev)
         fn = lambda: F.gqa_decode_attention_paged(q, kp, vp, table, lens, L)  # noqa: E731
+    elif args.profile_kv8:
+        B, L, ps = (int(v) for v in args.profile_kv8.split(","))
+        g = torch.Generator(device="cpu").manual_seed(1)
+        per = (L + ps - 1) // ps
+        cache = F.kv8_cache(B * per, 8, ps, device=dev)
+        table = torch.randperm(B * per, generator=g).to(torch.int32).view(B, per).to(dev)
+        inv_freq, _ = F.rope_inv_freq(128, device=dev)
+        rows = torch.randn((B * (L - 1), 16, 128), device=dev).to(torch.bfloat16)
+        F.kv8_append(rows[:, :8], rows[:, 8:], cache, table, torch.full((B,), L - 1, dtype=torch.int32, device=dev),
+                     inv_freq=inv_freq)
+        del rows
+        q, k, v = torch.randn((B, 48, 128), device=dev).to(torch.bfloat16).split([32, 8, 8], 1)
+        lens = torch.full((B,), L, dtype=torch.int32, device=dev)
+        fn = lambda: F.decode_attention_kv8(q, k, v, cache, table, lens, L, inv_freq)  # noqa: E731
     else:
         B, L = (int(v) for v in args.profile_attn.split(","))
         g = torch.Generator(device="cpu").manual_seed(1)
@@ -1027,6 +1043,7 @@ def main(argv=None):
     ap.add_argument("--profile-shape", default=None, help="M,K,N: only run a few calls (ncu)")
     ap.add_argument("--profile-attn", default=None, help="B,L: only run a few attention calls (ncu)")
     ap.add_argument("--profile-paged", default=None, help="B,L,page_size: a few paged attention calls (ncu)")
+    ap.add_argument("--profile-kv8", default=None, help="B,L,page_size: a few 8-bit cache decode steps (ncu)")
     ap.add_argument("--profile-sweep", action="store_true", help="each sweep shape once per call round (ncu)")
     ap.add_argument("--profile-calls", type=int, default=3)
     args = ap.parse_args(argv)
@@ -1036,7 +1053,7 @@ def main(argv=None):
     if args.timeline:
         run_timeline(args)
         return 0
-    if args.profile_shape or args.profile_attn or args.profile_sweep or args.profile_paged:
+    if args.profile_shape or args.profile_attn or args.profile_sweep or args.profile_paged or args.profile_kv8:
         run_profile_case(args)
         return 0
     if args.warmup < 3:

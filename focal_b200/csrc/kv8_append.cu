@@ -374,6 +374,7 @@ extern "C" int focal_kv8_append(const focal_kv8_append_args* a, const focal_kv8_
     return set_error(FOCAL_ERR_UNSUPPORTED, "unsupported dtype (must be bf16 or fp16)");
   if (a->B < 0 || a->T < 0 || a->max_new < 0 || a->Hq < 0 || a->max_pages_per_seq < 1)
     return set_error(FOCAL_ERR_UNSUPPORTED, "B, T, max_new and Hq must not be negative, max_pages_per_seq positive");
+  if (Hkv > 65535 || a->Hq > 65535) return set_error(FOCAL_ERR_UNSUPPORTED, "too many heads");
   if (!a->cu_new && (long long)a->B * a->max_new != a->T)
     return set_error(FOCAL_ERR_UNSUPPORTED, "without cu_new, T must be B * max_new");
   if (a->rot != 0 && (a->rot < 16 || a->rot % 16 != 0 || a->rot > D))

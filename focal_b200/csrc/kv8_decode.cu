@@ -8,16 +8,20 @@
 // Bound: HBM, by the codes (2 D bytes per position and KV head); the codes are
 // half of a bf16 cache's bytes, so an SM has half the time per position and the
 // work per code counts.
-//  * All tiles (kTile positions of one segment: a sequence, a KV head and up to 16
-//    query rows) of all sequences form one flat order, which is cut into
-//    equal ranges, one per CTA, and these into one per warp.  Lengths that
-//    differ, and numbers of segments that do not divide the SMs, cost nothing.
-//    Where a segment lies in several warps or CTAs its parts are joined by their
-//    log-sum-exp, in the flat order: in shared memory, then by the last CTA to arrive.
+//  * A segment is a sequence, a KV head and up to 16 query rows; its tiles have 64
+//    positions.  Where lengths are alike each segment gets whole CTAs (or a CTA
+//    whole segments), else the tiles of all segments, in one flat order, are cut into
+//    equal ranges, one per CTA; the kernel decides by the lengths it finds.  A
+//    CTA's range is cut into one per warp.  Parts of a segment in several warps or CTAs
+//    are joined by their log-sum-exp in the flat order: in shared memory, then by
+//    the last CTA to arrive.  (16 sequences of 16 tiles: 13.9 us cut evenly, with a join,
+//    11.7 by segments; 128 sequences of up to 2048: 92 us by segments, 55 evenly.)
 //  * Every warp streams its own tiles through a ring of its own: it issues the TMA
 //    boxes of a tile's K and V (swizzled) and the copies of its scales, kRing tiles
 //    ahead, into the slot it has just read.  No warp waits for another before
-//    the end, and a late box holds up one ring only.
+//    the end, and a late box holds up one ring only.  (One producer warp with a
+//    ring for all streamed at 0.56 of the measured copy rate, this at 1.04: 8 sequences of 131072
+//    tokens 591 and 317 us.)
 //  * The products are transposed: S^T = K Q^T and O^T = V^T P^T.  The 16-row side
 //    of mma.sync m16n8k16 holds positions and dims, its 8-column side the query rows
 //    (T * Hq / Hkv, 8 or 16 of them), which halves the products that 4 or 8
@@ -34,6 +38,9 @@
 //    (p >= 2^-29 keeps f16's 11 bits), vs is its block's V scale and R the smallest power
 //    of two >= the V scales seen by the warp so far, so vs / R <= 1; when R
 //    grows the accumulators are rescaled as they are when the maximum grows.
+// What is left: launch, lengths, page ids and the first tiles one after another
+// (about 4 us), and merge and join at the end (1 to 3 us); one sequence of 512
+// takes 6.4 us, 16 ragged ones of up to 4096 24.7 where their bytes take 11.4.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -50,7 +57,6 @@ constexpr int kRing = 2;                 // tiles of a warp's ring
 // Warps of a CTA: what fits into shared memory; for head_dim 64 (half the bytes
 // a tile, but the same softmax) as many as fit into the registers.
 __host__ __device__ constexpr int warps_of(int D) { return D == 128 ? 7 : 12; }
-constexpr int kMaxWarps = warps_of(64) > warps_of(128) ? warps_of(64) : warps_of(128);
 constexpr int kMaxQueryTokens = 16;
 constexpr int kMaxGroup = 16;
 constexpr int kRowsPerCta = 16;  // query rows of a segment
@@ -114,6 +120,10 @@ template <typename T>
 __device__ __forceinline__ void store4(T* p, float4 v) {
   *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
 }
+
+// Whether one of a word's four e4m3 codes is NaN (all seven bits behind the sign set), and the word without those.
+__device__ __forceinline__ bool has_nan_code(uint32_t w) { return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu) != 0; }
+__device__ __forceinline__ uint32_t no_nan_codes(uint32_t w) { return w & ~__vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
 
 // 2^e for e <= 127; 0 below the normal numbers
 __device__ __forceinline__ float exp2_int(int e) {
@@ -192,7 +202,7 @@ __global__ void __launch_bounds__(32 * warps_of(D))
   // kHbm for each of all tiles, a CTA kOwn for each of its own (measured with 128
   // CTAs at work), a join and what goes with it 2000 and 3500.
   constexpr float kHbm = D == 128 ? 4.8f : 2.4f;
-  constexpr int kOwn = (D == 128 ? 560 : 320) * (NT == 2 ? 5 : 4) / 4 * (INT8 ? 9 : 8) / 8;
+  constexpr float kOwn = (D == 128 ? 560.f : 320.f) * (NT == 2 ? 1.25f : 1.f) * (INT8 ? 1.125f : 1.f);
   const int cta = blockIdx.x;
   int ways = p.ways, per = p.per;
   int total = 0, len32 = 0;
@@ -211,16 +221,16 @@ __global__ void __launch_bounds__(32 * warps_of(D))
     empty = __any_sync(0xffffffffu, empty);
     total = __reduce_add_sync(0xffffffffu, total) * hc;
     top = __reduce_max_sync(0xffffffffu, top);
-    const int hbm = static_cast<int>(kHbm * total), even = max(4, p.by_grid(total + gridDim.x - 1));
-    const int evenly = max(hbm, kOwn * even) + 3500;
+    const int even = max(4, p.by_grid(total + gridDim.x - 1));
+    const float hbm = kHbm * total, evenly = fmaxf(hbm, kOwn * even) + 3500.f;
     if (ways > 0) {
       if (top <= kWarps * 3 / 2) ways = 1;
       const int part = ways == 1 ? top : p.by_ways(top + ways - 1);
       per = max(part, 1);
-      if (max(hbm, kOwn * part) + (ways > 1 ? 2000 : 0) > evenly) ways = 0;
+      if (fmaxf(hbm, kOwn * part) + (ways > 1 ? 2000.f : 0.f) > evenly) ways = 0;
     } else {
       per = 0;
-      if (total == p.segs * top && max(hbm, kOwn * p.stack * top) <= evenly) per = p.stack * top;
+      if (total == p.segs * top && fmaxf(hbm, kOwn * (p.stack * top)) <= evenly) per = p.stack * top;
     }
     if (ways == 0 && (p.ways > 0 || per == 0)) per = even;
   }
@@ -488,6 +498,37 @@ __global__ void __launch_bounds__(32 * warps_of(D))
       __syncwarp();
     }
 
+    if (!INT8 && edge && p.T > 1) {
+      // A NaN V code of a position that some rows see and others do not would reach all
+      // of them as 0 times NaN: it is put into the sums of those that see it, and zeroed.
+      const int from = max(lim_min - pos0, 0), to = min(clen - pos0, kTile);
+      bool bad = false;
+      for (int e = from * (D / 16) + lane; e < to * (D / 16); e += 32) {
+        const uint4 u = lds128(vt + S::at(e / (D / 16), e % (D / 16)));
+        bad |= has_nan_code(u.x) || has_nan_code(u.y) || has_nan_code(u.z) || has_nan_code(u.w);
+      }
+      if (__any_sync(0xffffffffu, bad)) {
+#pragma unroll 1
+        for (int e = from; e < to; ++e)
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            const uint32_t v = lds_u16(vt + S::at(e, c) + 2 * g);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if ((v >> (8 * (i >> 1)) & 0x7F) == 0x7F && pos0 + e < lim[n][i & 1]) acc[c][n][i] = NAN;
+          }
+        __syncwarp();
+        for (int e = from * (D / 16) + lane; e < to * (D / 16); e += 32) {
+          const uint32_t at = vt + S::at(e / (D / 16), e % (D / 16));
+          const uint4 u = lds128(at);
+          sts128(at, make_uint4(no_nan_codes(u.x), no_nan_codes(u.y), no_nan_codes(u.z), no_nan_codes(u.w)));
+        }
+        __syncwarp();
+      }
+    }
+
     // ---- S^T = K Q^T, 16 positions (one block of the cache) at a time
     float s[kBlocks][NT][4];
 #pragma unroll
@@ -654,7 +695,13 @@ __global__ void __launch_bounds__(32 * warps_of(D))
       load_q();
     }
   }
-  if (!ok) set_status(p.status, kDevWaitTimeout);
+  if (!ok) {  // a copy did not land in time: give those in flight their time before the CTA ends
+    set_status(p.status, kDevWaitTimeout);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_wait_bounded(full_bar + 8 * i, 0);
+      mbar_wait_bounded(full_bar + 8 * i, 1);
+    }
+  }
 
   // ---- merge the portions of each segment; a thread has one row's 4 dims
   Portion* parts = reinterpret_cast<Portion*>(sm + S::kParts);

@@ -202,7 +202,10 @@ extern "C" int focal_rope(const void* x, void* y, const void* positions, const d
       tokens = t;
     }
   }
-  if (tokens == 1 || T <= places) {
+  if (per_token * tokens > 1 << 24) {  // more heads than a block has a use for
+    tokens = 1;
+    heads = (int)std::min<long long>(H, (1 << 16) / items);
+  } else if (tokens == 1 || T <= places) {
     tokens = 1;
     const long long blocks = std::max<long long>(1, std::min<long long>(places / T, (per_token + rope::kThreads - 1) / rope::kThreads));
     heads = (int)((H + blocks - 1) / blocks);

@@ -138,6 +138,26 @@ def test_append_is_exact(cuda, code, dtype, H, D, page_size):
 
 
 @pytest.mark.parametrize("code", [E4M3, INT8])
+def test_append_behind_rows_with_any_scale(cuda, code):
+    """Blocks that something else filled, with scales that are no powers of two: some
+    grow, some keep their scale and are divided by it."""
+    H, D, S = 4, 64, 32
+    lens0, new = [5, 20, 31, 47, 10], [3, 1, 1, 1, 6]
+    table, pages = table_for([n + m for n, m in zip(lens0, new)], S, cuda, seed=6)
+    cache = random_cache(pages, H, S, D, code, cuda, seed=6)
+    mine = clones(cache)
+    lens = [n + m for n, m in zip(lens0, new)]
+    T = sum(new)
+    x = (torch.randn(T, H, D, device=cuda, generator=gen(cuda, 7)) *
+         torch.exp(2 * torch.randn(T, H, 1, device=cuda, generator=gen(cuda, 8)))).to(BF16)
+    cu = ints([sum(new[:b]) for b in range(6)], cuda)
+    F.kv8_append(x, -x, cache, table, ints(lens, cuda), cu_new=cu, max_new=6)
+    fp32_append(x, mine.k_pages, mine.k_scales, code, table, lens, new)
+    fp32_append(-x, mine.v_pages, mine.v_scales, code, table, lens, new)
+    assert same(cache, mine) and status() == 0
+
+
+@pytest.mark.parametrize("code", [E4M3, INT8])
 def test_append_extremes(cuda, code):
     """Zero blocks, the smallest and largest values, infinities and NaN, and a zero
     block that grows later."""
@@ -367,6 +387,30 @@ def test_attention_nan_where_it_is_seen(cuda):
     got = F.gqa_decode_attention_kv8(q, cache, table, ints([200, 200], cuda), 200)
     bad = torch.isnan(got)
     assert torch.all(bad[0, 4:]) and not torch.any(bad[0, :4]) and not torch.any(bad[1])
+
+
+@pytest.mark.parametrize("D,Hq,H", [(128, 8, 2), (64, 16, 1)])
+def test_attention_nan_that_some_queries_see(cuda, D, Hq, H):
+    """NaN values among the newest positions: the queries before them do not see them, the
+    others do in those dims only."""
+    T, n = 5, 200
+    table, pages = table_for([n, 64], 32, cuda, seed=5)
+    cache = random_cache(pages, H, 32, D, E4M3, cuda, seed=5)
+    q = torch.randn(2, T, Hq, D, device=cuda, generator=gen(cuda, 6)).to(BF16)
+    lens = ints([n, 64], cuda)
+    clean = ok.attention(q, doubles(cache), table.cpu(), [n, 64])
+    raw = cache.v_pages.view(torch.uint8)
+    for pos, d in ((n - 2, 7), (n - 2, 8), (n - 1, 40)):  # seen by t >= 3, t >= 3 and t = 4
+        raw[table[0, pos // 32], 0, pos % 32, d] = 0xFF if d == 8 else 0x7F
+    got = F.gqa_decode_attention_kv8(q, cache, table, lens, n)
+    want = torch.zeros(2, T, Hq, D, dtype=torch.bool, device=cuda)
+    want[0, 3:, :Hq // H, 7:9] = True
+    want[0, 4:, :Hq // H, 40] = True
+    assert torch.equal(torch.isnan(got), want)
+    free = torch.ones_like(want)
+    free[0, 3:, :Hq // H] = False  # (the others also miss nothing but the NaN codes)
+    tol = attention_tolerance(clean, BF16, D)
+    assert torch.all(((got.double() - clean[0]).abs() <= tol)[free])
 
 
 def test_attention_is_deterministic_and_shares_pages(cuda):

@@ -16,12 +16,14 @@
 //    are joined by their log-sum-exp in the flat order: in shared memory, then by
 //    the last CTA to arrive.  (16 sequences of 16 tiles: 13.9 us cut evenly, with a join,
 //    11.7 by segments; 128 sequences of up to 2048: 92 us by segments, 55 evenly.)
-//  * Every warp streams its own tiles through a ring of its own: it issues the TMA
-//    boxes of a tile's K and V (swizzled) and the copies of its scales, kRing tiles
-//    ahead, into the slot it has just read.  No warp waits for another before
-//    the end, and a late box holds up one ring only.  (One producer warp with a
-//    ring for all streamed at 0.56 of the measured copy rate, this at 1.04: 8 sequences of 131072
-//    tokens 591 and 317 us.)
+//  * Every warp streams its own tiles through a ring of its own, three half tiles:
+//    into the slot of K or V that it has just read it issues the TMA boxes (swizzled)
+//    of the half tile three places on; the blocks' scales come by plain loads into
+//    registers.  No warp waits for another before the end, and a late box holds up
+//    one ring only.  (One producer warp with a ring for all streamed at 0.56 of the
+//    measured copy rate, this at 1.04: 8 sequences of 131072 tokens 591 and 317 us.  Seven
+//    warps with two whole tiles each, which left one scheduler half idle and HBM waiting for
+//    the first tiles' work: 16 ragged sequences 24.6 us instead of 21.9.)
 //  * The products are transposed: S^T = K Q^T and O^T = V^T P^T.  The 16-row side
 //    of mma.sync m16n8k16 holds positions and dims, its 8-column side the query rows
 //    (T * Hq / Hkv, 8 or 16 of them), which halves the products that 4 or 8
@@ -40,7 +42,7 @@
 //    grows the accumulators are rescaled as they are when the maximum grows.
 // What is left: launch, lengths, page ids and the first tiles one after another
 // (about 4 us), and merge and join at the end (1 to 3 us); one sequence of 512
-// takes 6.4 us, 16 ragged ones of up to 4096 24.7 where their bytes take 11.4.
+// takes 5.8 us, 16 ragged ones of up to 4096 21.9 where their bytes take 11.4.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -53,10 +55,11 @@ namespace kv8 {
 constexpr int kTile = 64;  // positions of a tile
 constexpr int kTileBits = 6;
 constexpr int kBlocks = kTile / kGroup;  // blocks of the cache (scales) in a tile
-constexpr int kRing = 2;                 // tiles of a warp's ring
-// Warps of a CTA: what fits into shared memory; for head_dim 64 (half the bytes
-// a tile, but the same softmax) as many as fit into the registers.
-__host__ __device__ constexpr int warps_of(int D) { return D == 128 ? 7 : 12; }
+constexpr int kRing = 3;                 // a warp's ring: a tile's K, its V, the next tile's K
+// Warps of a CTA: what fits into shared memory, the same number on each of the SM's four
+// schedulers (with 7, the warp that had one to itself was through a fifth sooner); for head_dim
+// 64 (half the bytes a tile, but the same softmax) as many as fit into the registers.
+__host__ __device__ constexpr int warps_of(int D) { return D == 128 ? 8 : 12; }
 constexpr int kMaxQueryTokens = 16;
 constexpr int kMaxGroup = 16;
 constexpr int kRowsPerCta = 16;  // query rows of a segment
@@ -93,8 +96,7 @@ template <int D>
 struct Smem {
   static constexpr int kWarps = warps_of(D);
   static constexpr int kTileBytes = kTile * D;
-  static constexpr int kSlotBytes = 2 * kTileBytes;
-  static constexpr int kWarpBytes = kRing * kSlotBytes;  // a warp's ring, and at the end its last portion's record
+  static constexpr int kWarpBytes = kRing * kTileBytes;  // a warp's ring, and at the end its last portion's record
   static constexpr int kPortions = kWarps * kWarpBytes;  // Portion [warp][first, last]
   static constexpr int kParts = kPortions + kWarps * 2 * 12;  // Portion [2]: what cta_rec got
   static constexpr int kLast = kParts + 2 * 12;               // int [2]
@@ -202,7 +204,7 @@ __global__ void __launch_bounds__(32 * warps_of(D))
   // kHbm for each of all tiles, a CTA kOwn for each of its own (measured with 128
   // CTAs at work), a join and what goes with it 2000 and 3500.
   constexpr float kHbm = D == 128 ? 4.8f : 2.4f;
-  constexpr float kOwn = (D == 128 ? 560.f : 320.f) * (NT == 2 ? 1.25f : 1.f) * (INT8 ? 1.125f : 1.f);
+  constexpr float kOwn = (D == 128 ? 520.f : 330.f) * (NT == 2 ? 1.25f : 1.f) * (INT8 ? 1.2f : 1.f);
   const int cta = blockIdx.x;
   int ways = p.ways, per = p.per;
   int total = 0, len32 = 0;
@@ -335,12 +337,26 @@ __global__ void __launch_bounds__(32 * warps_of(D))
     }
   };
   int ids = 0, rows_in = 0, whats = 0, chunk = -1;
-  // The scales of the tiles in flight, oldest first: lanes 0 .. kBlocks - 1 have K's, the next kBlocks V's.
-  float scale_in[kRing];
-#pragma unroll
-  for (int i = 0; i < kRing; ++i) scale_in[i] = 0.f;
-  // The whole warp: start the loads of its j-th tile into slot j % kRing, and of its scales into `mine`.
-  auto issue = [&](int j, float& mine) {
+  // The scales of the tiles in flight, this one's and the next's: lanes 0 .. kBlocks - 1 have K's, the next kBlocks V's.
+  float scale_in[2] = {0.f, 0.f};
+  // The whole warp: start the load of its j-th tile's K or V into a slot of the ring.
+  auto issue = [&](int j, int slot, int r, int what, const CUtensorMap* map) {
+    const uint32_t fb = full_bar + 8 * slot, dst = ring + slot * S::kTileBytes;
+    const int n = what & 7, kvh = what >> 3;
+    const int id = __shfl_sync(0xffffffffu, ids, ((j << page_bits) + lane) & 31);
+    if (page_bits == 0) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(fb, S::kTileBytes);
+        tma_load_4d(dst, map, 0, r, kvh, id, fb, pol);
+      }
+    } else {
+      if (lane == 0) mbar_arrive_expect_tx(fb, n * box * D);
+      __syncwarp();
+      if (lane < n) tma_load_4d(dst + lane * box * D, map, 0, r, kvh, id, fb, pol);
+    }
+  };
+  // K of tile j, and its scales into `mine`
+  auto issue_k = [&](int j, int slot, float& mine) {
     if (j >= nj) return;
     const bool fresh = (j >> chunk_bits) != chunk;
     if (fresh) {
@@ -353,32 +369,21 @@ __global__ void __launch_bounds__(32 * warps_of(D))
         ids = 0;
       }
     }
-    const int slot = j % kRing;
-    const uint32_t fb = full_bar + 8 * slot, dst = ring + slot * S::kSlotBytes;
     const int src = (j << page_bits) & 31;
-    const int blk = lane % kBlocks, pg = (blk * kGroup) >> box_bits;  // this lane's block and its page in the tile
     const int what = __shfl_sync(0xffffffffu, whats, src), r = __shfl_sync(0xffffffffu, rows_in, src);
-    const int id = __shfl_sync(0xffffffffu, ids, (src + lane) & 31);
-    const int gid = __shfl_sync(0xffffffffu, ids, (src + pg) & 31);
-    const int n = what & 7, kvh = what >> 3;
-    if (page_bits == 0) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(fb, S::kSlotBytes);
-        tma_load_4d(dst, &tmap_k, 0, r, kvh, id, fb, pol);
-        tma_load_4d(dst + S::kTileBytes, &tmap_v, 0, r, kvh, id, fb, pol);
-      }
-    } else {
-      if (lane == 0) mbar_arrive_expect_tx(fb, n * 2 * box * D);
-      __syncwarp();
-      if (lane < n) {
-        tma_load_4d(dst + lane * box * D, &tmap_k, 0, r, kvh, id, fb, pol);
-        tma_load_4d(dst + S::kTileBytes + lane * box * D, &tmap_v, 0, r, kvh, id, fb, pol);
-      }
-    }
-    if (lane < 2 * kBlocks && pg < n)
-      mine = (lane < kBlocks ? p.k_scales : p.v_scales)[((size_t)gid * p.Hkv + kvh) * groups +
+    issue(j, slot, r, what, &tmap_k);
+    const int blk = lane % kBlocks, pg = (blk * kGroup) >> box_bits;  // this lane's block and its page in the tile
+    const int id = __shfl_sync(0xffffffffu, ids, (src + pg) & 31);
+    if (lane < 2 * kBlocks && pg < (what & 7))
+      mine = (lane < kBlocks ? p.k_scales : p.v_scales)[((size_t)id * p.Hkv + (what >> 3)) * groups +
                                                         (r / kGroup + blk - (pg << box_bits) / kGroup)];
     if (fresh && ((chunk + 1) << chunk_bits) < nj) load_chunk(chunk + 1);  // looked at a chunk later
+  };
+  // V of tile j (its K was issued after the V before it, so the chunk is its own)
+  auto issue_v = [&](int j, int slot) {
+    if (j >= nj) return;
+    const int src = (j << page_bits) & 31;
+    issue(j, slot, __shfl_sync(0xffffffffu, rows_in, src), __shfl_sync(0xffffffffu, whats, src), &tmap_v);
   };
   load_chunk(0);
 
@@ -406,8 +411,9 @@ __global__ void __launch_bounds__(32 * warps_of(D))
     }
   };
   if (nj > 0) load_q();
-#pragma unroll
-  for (int j = 0; j < kRing; ++j) issue(j, scale_in[j]);
+  issue_k(0, 0, scale_in[0]);
+  issue_v(0, 1);
+  issue_k(1, 2, scale_in[1]);
 
   float rowf[NT][2];  // scores to log2 units, for rows 2t and 2t + 1 of a tile of 8
   int lim[NT][2];     // positions that they see
@@ -417,6 +423,14 @@ __global__ void __launch_bounds__(32 * warps_of(D))
   int vexp = -126;         // log2 R
   bool begins = true;      // a portion begins with this tile
   bool ok = true;
+  // K of tile j is load 2j of this warp, V load 2j + 1: load i is in slot i % 3, its phase i / 3
+  int slot = 0, phase = 0;
+  auto next_slot = [&]() {
+    if (++slot == kRing) {
+      slot = 0;
+      phase ^= 1;
+    }
+  };
 
   // The portion's state as a record
   auto emit_record = [&](float* rec) {
@@ -473,12 +487,11 @@ __global__ void __launch_bounds__(32 * warps_of(D))
         }
       }
     }
-    const int slot = j % kRing;
-    if (!mbar_wait_bounded(full_bar + 8 * slot, (j / kRing) & 1)) {
+    if (!mbar_wait_bounded(full_bar + 8 * slot, phase)) {
       ok = false;
       break;
     }
-    const uint32_t kt = ring + slot * S::kSlotBytes, vt = kt + S::kTileBytes;
+    const uint32_t kt = ring + slot * S::kTileBytes;
     const int pos0 = ct * kTile;
     const bool edge = pos0 + kTile > lim_min;  // some row does not see all of the tile
     float ks[kBlocks], vs[kBlocks];
@@ -487,46 +500,10 @@ __global__ void __launch_bounds__(32 * warps_of(D))
       ks[m] = __shfl_sync(0xffffffffu, scale_in[0], m);
       vs[m] = __shfl_sync(0xffffffffu, scale_in[0], kBlocks + m);
     }
-    if (pos0 + kTile > clen) {
-      // V rows past the end may hold anything (NaN times p = 0 would still be NaN), and so may their blocks' scales
-      const int left = clen - pos0;
-      for (int e = left * (D / 16) + lane; e < kTile * (D / 16); e += 32)
-        sts128(vt + S::at(e / (D / 16), e % (D / 16)), make_uint4(0u, 0u, 0u, 0u));
+    if (pos0 + kTile > clen) {  // blocks past the end may have any scale
 #pragma unroll
       for (int m = 1; m < kBlocks; ++m)
-        if (left <= kGroup * m) vs[m] = 0.f;
-      __syncwarp();
-    }
-
-    if (!INT8 && edge && p.T > 1) {
-      // A NaN V code of a position that some rows see and others do not would reach all
-      // of them as 0 times NaN: it is put into the sums of those that see it, and zeroed.
-      const int from = max(lim_min - pos0, 0), to = min(clen - pos0, kTile);
-      bool bad = false;
-      for (int e = from * (D / 16) + lane; e < to * (D / 16); e += 32) {
-        const uint4 u = lds128(vt + S::at(e / (D / 16), e % (D / 16)));
-        bad |= has_nan_code(u.x) || has_nan_code(u.y) || has_nan_code(u.z) || has_nan_code(u.w);
-      }
-      if (__any_sync(0xffffffffu, bad)) {
-#pragma unroll 1
-        for (int e = from; e < to; ++e)
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            const uint32_t v = lds_u16(vt + S::at(e, c) + 2 * g);
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if ((v >> (8 * (i >> 1)) & 0x7F) == 0x7F && pos0 + e < lim[n][i & 1]) acc[c][n][i] = NAN;
-          }
-        __syncwarp();
-        for (int e = from * (D / 16) + lane; e < to * (D / 16); e += 32) {
-          const uint32_t at = vt + S::at(e / (D / 16), e % (D / 16));
-          const uint4 u = lds128(at);
-          sts128(at, make_uint4(no_nan_codes(u.x), no_nan_codes(u.y), no_nan_codes(u.z), no_nan_codes(u.w)));
-        }
-        __syncwarp();
-      }
+        if (clen - pos0 <= kGroup * m) vs[m] = 0.f;
     }
 
     // ---- S^T = K Q^T, 16 positions (one block of the cache) at a time
@@ -551,6 +528,11 @@ __global__ void __launch_bounds__(32 * warps_of(D))
         }
       }
     }
+    // K's slot is read: the next tile's V goes there
+    fence_proxy_async_smem();
+    __syncwarp();
+    issue_v(j + 1, slot);
+    next_slot();
     // ---- scale, mask, tile maximum
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -613,6 +595,48 @@ __global__ void __launch_bounds__(32 * warps_of(D))
         }
       }
     }
+    if (!mbar_wait_bounded(full_bar + 8 * slot, phase)) {
+      ok = false;
+      break;
+    }
+    const uint32_t vt = ring + slot * S::kTileBytes;
+    if (pos0 + kTile > clen) {
+      // V rows past the end may hold anything, and NaN times p = 0 would still be NaN
+      for (int e = (clen - pos0) * (D / 16) + lane; e < kTile * (D / 16); e += 32)
+        sts128(vt + S::at(e / (D / 16), e % (D / 16)), make_uint4(0u, 0u, 0u, 0u));
+      __syncwarp();
+    }
+
+    if (!INT8 && edge && p.T > 1) {
+      // A NaN V code of a position that some rows see and others do not would reach all
+      // of them as 0 times NaN: it is put into the sums of those that see it, and zeroed.
+      const int from = max(lim_min - pos0, 0), to = min(clen - pos0, kTile);
+      bool bad = false;
+      for (int e = from * (D / 16) + lane; e < to * (D / 16); e += 32) {
+        const uint4 u = lds128(vt + S::at(e / (D / 16), e % (D / 16)));
+        bad |= has_nan_code(u.x) || has_nan_code(u.y) || has_nan_code(u.z) || has_nan_code(u.w);
+      }
+      if (__any_sync(0xffffffffu, bad)) {
+#pragma unroll 1
+        for (int e = from; e < to; ++e)
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            const uint32_t v = lds_u16(vt + S::at(e, c) + 2 * g);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if ((v >> (8 * (i >> 1)) & 0x7F) == 0x7F && pos0 + e < lim[n][i & 1]) acc[c][n][i] = NAN;
+          }
+        __syncwarp();
+        for (int e = from * (D / 16) + lane; e < to * (D / 16); e += 32) {
+          const uint32_t at = vt + S::at(e / (D / 16), e % (D / 16));
+          const uint4 u = lds128(at);
+          sts128(at, make_uint4(no_nan_codes(u.x), no_nan_codes(u.y), no_nan_codes(u.z), no_nan_codes(u.w)));
+        }
+        __syncwarp();
+      }
+    }
     // ---- weights, and O^T += V^T P^T
 #pragma unroll
     for (int m = 0; m < kBlocks; ++m) {
@@ -642,11 +666,11 @@ __global__ void __launch_bounds__(32 * warps_of(D))
         for (int n = 0; n < NT; ++n) mma_f16_16816(acc[c + 1][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
       }
     }
-    fence_proxy_async_smem();  // our reads and zeros of this slot precede its refill
+    fence_proxy_async_smem();  // our reads and zeros of V's slot precede its refill, the K after next
     __syncwarp();
-#pragma unroll
-    for (int i = 0; i + 1 < kRing; ++i) scale_in[i] = scale_in[i + 1];
-    issue(j + kRing, scale_in[kRing - 1]);
+    scale_in[0] = scale_in[1];
+    issue_k(j + 2, slot, scale_in[1]);
+    next_slot();
 
     // ---- the end of a portion
     const int n_tiles = tiles_of(clen);

@@ -18,17 +18,19 @@
 // does lose precision with a scale larger than needed, so it takes amax / 127 and pays
 // one more rounding when a block grows.
 //
-// One warp takes one (block, head) of K or of V, or 16 rows of one query head:
-// a lane holds 16 dims of every (32 / (D / 16))-th row in fp32 registers, so the
-// rows are read once and amax needs one warp reduction; the next job's rows are
-// on their way to shared memory meanwhile.  The cos and sin of the
-// block's rows are computed once per thread block into shared memory: of many
-// rows, eight follow from one angle by turning it on by inv_freq in 64 bits.
+// One warp takes one (block, head) of K or of V, or 16 rows of one query head, while
+// the next job's rows are on their way to shared memory; a lane has 16 dims of
+// every (32 / (D / 16))-th row.  K and V pass over their rows twice, for amax and for
+// the codes, from shared memory.  The cos and sin of the block's rows are computed
+// once per thread block into shared memory: of many rows, eight follow from one angle by
+// turning it on by inv_freq in 64 bits.
 //
-// Bound: HBM and the issue of about 600 instructions a job for prompts (8 x 1024
-// tokens of 32 + 16 heads 38.4 us, 0.73 of the measured copy rate), the chain of
-// dependent loads (length, then page and rows) for a step (8 tokens 4.1 us),
-// whose heads are spread over thread blocks.
+// Bound: HBM and the issue of some 800 instructions a job for prompts (8 x 1024
+// tokens of 32 + 16 heads 34.2 us, 0.83 of the measured copy rate; 5072 tokens in
+// five prompts 22.8 us, 0.77), the chain of dependent loads (length, then page and
+// rows) for a step (8 tokens 3.5 us), whose heads are spread over thread blocks.
+// Measured against it: the 64 values of a lane held in registers between
+// the two passes, 8 warps a thread block, two blocks an SM: 38.4 and 30.3 us.
 #include <algorithm>
 #include <cmath>
 
@@ -37,7 +39,8 @@
 namespace focal {
 namespace kv8 {
 
-constexpr int kAppendWarps = 8;
+constexpr int kAppendWarps = 4;
+constexpr int kBlocksPerSm = 5;  // what shared memory holds
 
 struct AppendParams {
   const void *k, *v, *q;
@@ -119,10 +122,9 @@ __device__ __forceinline__ void dequantise4(uint32_t c, float (&x)[4]) {
 }
 
 template <typename T, int D, bool INT8, bool INTERLEAVED>
-__global__ void __launch_bounds__(32 * kAppendWarps, 2) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(32 * kAppendWarps, kBlocksPerSm) append_kernel(const AppendParams p) {
   constexpr int kLanes = D / 16;      // lanes of one row
   constexpr int kRows = 32 / kLanes;  // rows that a warp holds side by side
-  constexpr int kPasses = kGroup / kRows;
   constexpr int kJobBytes = kGroup * D * 2;  // 16 rows of a head
   extern __shared__ __align__(16) uint8_t sm[];
   // cos and sin of row r and frequency f: a lane reads 8 frequencies, two at a time, side by side with its neighbours
@@ -218,46 +220,41 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 2) append_kernel(const Appe
     const long long ph = (long long)page * p.Hkv + h;
     float* sp = (is_v ? p.v_scales : p.k_scales) + ph * (p.page_size / kGroup) + sub / kGroup;
     const float old = !is_q && r0 > 0 ? *sp : 0.f;
-    // rows i * kRows .. of pass i: warps skip the passes without new rows
-    auto has = [&](int i) { return (i + 1) * kRows > r0 && i * kRows < r1; };
     cp_async_wait<1>();
     __syncwarp();
     const uint8_t* x = mine + slot * kJobBytes + rr * D * 2;
-    float val[kPasses][16];
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      if (!has(i)) continue;
+    // this lane's 16 values of pass i, turned if they are keys or queries
+    auto values = [&](int i, float (&val)[16]) {
       const uint4 u = *reinterpret_cast<const uint4*>(x + i * kRows * D * 2 + d0 * 2);
       const uint4 w = *reinterpret_cast<const uint4*>(x + i * kRows * D * 2 + d1 * 2);
       const uint32_t raw[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float2 f = unpack2<T>(raw[e]);
-        val[i][2 * e] = f.x;
-        val[i][2 * e + 1] = f.y;
+        val[2 * e] = f.x;
+        val[2 * e + 1] = f.y;
       }
-      if (!is_v && turns) {  // (rows of the pass that are not new hold anything, and are not used)
+      if (!is_v && turns) {
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
           const float4 a = *reinterpret_cast<const float4*>(cs + cs_at(i * kRows + rr, 8 * c + e));
-          rope_turn(INTERLEAVED ? val[i][2 * e] : val[i][e], INTERLEAVED ? val[i][2 * e + 1] : val[i][8 + e],
-                    make_float2(a.x, a.y));
-          rope_turn(INTERLEAVED ? val[i][2 * e + 2] : val[i][e + 1], INTERLEAVED ? val[i][2 * e + 3] : val[i][9 + e],
-                    make_float2(a.z, a.w));
+          rope_turn(val[INTERLEAVED ? 2 * e : e], val[INTERLEAVED ? 2 * e + 1 : 8 + e], make_float2(a.x, a.y));
+          rope_turn(val[INTERLEAVED ? 2 * e + 2 : e + 1], val[INTERLEAVED ? 2 * e + 3 : 9 + e], make_float2(a.z, a.w));
         }
       }
-    }
+    };
+    float val[16];
     if (is_q) {
       T* y = static_cast<T*>(p.q_out) + ((long long)(tok + rr) * p.Hq + h) * D;
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
+#pragma unroll 1
+      for (int i = r0 / kRows; i * kRows < r1; ++i) {
         const int r = i * kRows + rr;
+        values(i, val);
         if (r >= r0 && r < r1) {
           T* row = y + (long long)i * kRows * p.Hq * D;
           uint32_t w[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = pack2<T>(val[i][2 * e], val[i][2 * e + 1]);
+          for (int e = 0; e < 8; ++e) w[e] = pack2<T>(val[2 * e], val[2 * e + 1]);
           *reinterpret_cast<uint4*>(row + d0) = make_uint4(w[0], w[1], w[2], w[3]);
           *reinterpret_cast<uint4*>(row + d1) = make_uint4(w[4], w[5], w[6], w[7]);
         }
@@ -265,26 +262,26 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 2) append_kernel(const Appe
       __syncwarp();  // the buffer is read: the next job's fetch may fill it
       continue;
     }
-    // infinities saturate and NaN is stored as NaN (e4m3) or 0 (int8); neither sets the scale
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int r = i * kRows + rr;
-      if (has(i) && r >= r0 && r < r1) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(val[i][e]));  // not NaN
-      }
-    }
-    if (__any_sync(0xffffffffu, amax == INFINITY)) {
-      amax = 0.f;
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
+    // Twice over the rows, for amax and for the codes: turning them again costs less than
+    // the registers that would hold them.  Infinities saturate and NaN is stored as NaN
+    // (e4m3) or 0 (int8); neither sets the scale.
+    float amax = 0.f;
+#pragma unroll 1
+    for (int finite = 0; finite < 2; ++finite) {
+#pragma unroll 1
+      for (int i = r0 / kRows; i * kRows < r1; ++i) {
         const int r = i * kRows + rr;
-        if (r >= r0 && r < r1) {
+        values(i, val);
+        float m = 0.f;
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (fabsf(val[i][e]) < INFINITY) amax = fmaxf(amax, fabsf(val[i][e]));
+        for (int e = 0; e < 16; ++e) {
+          if (finite && !(fabsf(val[e]) < INFINITY)) val[e] = 0.f;
+          m = fmaxf(m, fabsf(val[e]));  // not NaN
         }
+        if (r >= r0 && r < r1) amax = fmaxf(amax, m);
       }
+      if (!__any_sync(0xffffffffu, amax == INFINITY)) break;
+      amax = 0.f;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
@@ -293,6 +290,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 2) append_kernel(const Appe
     const float inv = scale > 0.f ? 1.f / scale : 0.f;
     const bool exact = (__float_as_uint(scale) & 0x7FFFFFu) == 0;
     if (r0 > 0 && scale > old) {
+#pragma unroll 1
       for (int i = lane; i < r0 * (D / 4); i += 32) {  // four codes at a time
         uint32_t* a = reinterpret_cast<uint32_t*>(out) + i;
         float f[4];
@@ -302,14 +300,15 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 2) append_kernel(const Appe
         *a = quantise4<INT8>(f, scale, inv, exact);
       }
     }
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
+#pragma unroll 1
+    for (int i = r0 / kRows; i * kRows < r1; ++i) {
       const int r = i * kRows + rr;
-      if (has(i) && r >= r0 && r < r1) {
+      values(i, val);
+      if (r >= r0 && r < r1) {
         uint32_t w[4] = {0u, 0u, 0u, 0u};
         if (scale > 0.f) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = quantise4<INT8>(val[i] + 4 * e, scale, inv, exact);
+          for (int e = 0; e < 4; ++e) w[e] = quantise4<INT8>(val + 4 * e, scale, inv, exact);
         }
         *reinterpret_cast<uint2*>(out + r * D + d0) = make_uint2(w[0], w[1]);
         *reinterpret_cast<uint2*>(out + r * D + d1) = make_uint2(w[2], w[3]);
@@ -428,11 +427,11 @@ extern "C" int focal_kv8_append(const focal_kv8_append_args* a, const focal_kv8_
   p.pieces = static_cast<int>(pieces);
   p.mscale = a->mscale;
   // Heads of a block of tokens are spread over thread blocks until these are
-  // three to an SM (every one of them computes cos and sin anew).
+  // eight to an SM (every one of them computes cos and sin anew).
   const int jobs = 2 * Hkv + a->Hq;
   const long long blocks = std::min<long long>(pieces * a->B, (long long)a->T / kGroup + a->B);
   const int spread = (int)std::min<long long>((jobs + kAppendWarps - 1) / kAppendWarps,
-                                              std::max<long long>(1, (3LL * dev.sm_count + blocks - 1) / blocks));
+                                              std::max<long long>(1, (8LL * dev.sm_count + blocks - 1) / blocks));
   p.jobs_per_block = ((jobs + spread - 1) / spread + kAppendWarps - 1) / kAppendWarps * kAppendWarps;
   const dim3 grid(static_cast<unsigned>(pieces * a->B), (jobs + p.jobs_per_block - 1) / p.jobs_per_block, 1);
   const bool il = a->interleaved != 0;

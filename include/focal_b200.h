@@ -309,7 +309,7 @@ typedef struct focal_kv8_cache {
  * elements (multiples of 16 bytes), 16-byte aligned; q_out [T, Hq, head_dim]
  * contiguous; rot 0 or a multiple of 16 up to head_dim; Hq = 0 without q.
  * A length, cu_new entry or page id out of range sets device status 3, and
- * nothing is written for that sequence (or block). */
+ * nothing is written for that sequence (or block), its rows of q_out among it. */
 typedef struct focal_kv8_append_args {
   const void *k, *v, *q;
   void* q_out;
@@ -328,7 +328,10 @@ int focal_kv8_append(const focal_kv8_append_args* args, const focal_kv8_cache* c
  * fp32 scores, softmax and accumulation; split over the positions with a
  * log-sum-exp combine in split order.  A query that sees no position gives 0.
  * seq_lens[b] is 0 .. max_seq_len <= max_pages_per_seq * page_size (block
- * table entries and rows past a sequence's end are not read as data).
+ * table entries and rows past a sequence's end are not read as data).  Scales
+ * must not be negative.  Which tiles are summed together depends on the whole batch's
+ * lengths, so a sequence's result may differ in its last bits between batches;
+ * equal calls give equal bits.
  * Contract: Hq % num_kv_heads == 0, Hq / num_kv_heads <= 16, 1 <= T <= 16.
  *
  * Workspace: focal_kv8_decode_workspace_size() bytes, 256-byte aligned; its

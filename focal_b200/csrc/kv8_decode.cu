@@ -64,7 +64,10 @@ constexpr int kMaxQueryTokens = 16;
 constexpr int kMaxGroup = 16;
 constexpr int kRowsPerCta = 16;  // query rows of a segment
 constexpr int kMaxCtas = 256;
-constexpr int kCounterBytes = 256;  // granularity of the counters' region
+// One counter per CTA, not per segment: of the segments in several CTAs no two have the
+// same first one.  So the counters lie in the same place for calls of all shapes, and stay
+// zero between calls that share a workspace.
+constexpr int kCounterBytes = kMaxCtas * 4;
 constexpr int kBatch = 16;  // records whose loads a join has in flight
 constexpr int kJoin = 4;    // ways that many records are shared out
 constexpr float kWeightUp = 32768.f;
@@ -76,7 +79,7 @@ struct DecodeParams {
   const int32_t *block_table, *seq_lens;
   float* first_rec;        // [CTA][warp] records of portions that a warp left behind for its next segment
   float* cta_rec;          // [CTA][2] records of segments that come from, or go on into, another CTA
-  unsigned int* counters;  // [B][Hkv][chunks]
+  unsigned int* counters;  // [CTA]: arrivals at the segment that goes on from it into the next
   int* status;
   int B, T, Hq, Hkv, grp, chunks, num_pages, page_size, max_pages, max_len;
   // By segments: segs of them, `ways` CTAs each (0: more segments than CTAs) with
@@ -803,7 +806,7 @@ __global__ void __launch_bounds__(32 * warps_of(D))
     const Portion seg = parts[threadIdx.x];
     int c0;
     const unsigned int others = ctas_of(seg, c0) - 1;
-    last[threadIdx.x] = atom_add_acq_rel_gpu(p.counters + seg.seg, 1u) == others;
+    last[threadIdx.x] = atom_add_acq_rel_gpu(p.counters + c0, 1u) == others;
   }
   __syncthreads();
   for (int part = 0; part < 2; ++part) {
@@ -892,7 +895,7 @@ __global__ void __launch_bounds__(32 * warps_of(D))
       }
       __syncthreads();
     }
-    if (threadIdx.x == 0) p.counters[seg.seg] = 0u;  // zero again for the next call
+    if (threadIdx.x == 0) p.counters[c0] = 0u;  // zero again for the next call
   }
 }
 
@@ -911,17 +914,12 @@ int check_decode(int B, int T, int Hq, int Hkv, int max_seq_len, int D) {
   return FOCAL_OK;
 }
 
-size_t counter_bytes(int B, int T, int Hq, int Hkv) {
-  const size_t n = (size_t)B * Hkv * row_chunks(T, Hq, Hkv) * 4;
-  return (n + kCounterBytes - 1) / kCounterBytes * kCounterBytes;
-}
-
-// Records: one per warp and two per CTA.
+// Counters, and records: one per warp and two per CTA.
 size_t decode_workspace(int B, int T, int Hq, int Hkv, int max_seq_len, int D) {
   const size_t tiles = ((size_t)max_seq_len - 1) / kTile + 1;
   const size_t ctas = std::min<size_t>(kMaxCtas, tiles * B * Hkv * row_chunks(T, Hq, Hkv));
   const size_t rows = T * (Hq / Hkv) <= 8 ? 8 : 16;
-  return counter_bytes(B, T, Hq, Hkv) + ctas * (warps_of(D) + 2) * rows * (D + 10) * 4;
+  return kCounterBytes + ctas * (warps_of(D) + 2) * rows * (D + 10) * 4;
 }
 
 int check_cache(const focal_kv8_cache* c);
@@ -955,10 +953,7 @@ using namespace focal;
 
 extern "C" {
 
-size_t focal_kv8_decode_counter_bytes(int B, int T, int Hq, int Hkv) {
-  if (kv8::check_decode(B, T, Hq, Hkv, 1, 128)) return 0;
-  return kv8::counter_bytes(B, T, Hq, Hkv);
-}
+size_t focal_kv8_decode_counter_bytes(void) { return kv8::kCounterBytes; }
 
 size_t focal_kv8_decode_workspace_size(int B, int T, int Hq, int Hkv, int max_seq_len, int D) {
   if (kv8::check_decode(B, T, Hq, Hkv, max_seq_len, D)) return 0;
@@ -1023,7 +1018,7 @@ int focal_kv8_decode(const void* q, void* o, const focal_kv8_cache* cache, const
   p.seq_lens = seq_lens;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.counters = reinterpret_cast<unsigned int*>(ws);
-  p.cta_rec = reinterpret_cast<float*>(ws + counter_bytes(B, T, Hq, Hkv));
+  p.cta_rec = reinterpret_cast<float*>(ws + kCounterBytes);
   p.first_rec = p.cta_rec + (size_t)ctas * 2 * (T * (Hq / Hkv) <= 8 ? 8 : 16) * (D + 10);
   p.status = dev.status;
   p.B = B;

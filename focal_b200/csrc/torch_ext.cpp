@@ -549,8 +549,7 @@ torch::Tensor gqa_decode_attention_kv8(torch::Tensor q, torch::Tensor k_pages, t
   void* ws = nullptr;
   torch::Tensor ws_t;
   if (bytes > 0) {
-    ws_t = capturable_workspace(kWsKv8, q.device(), stream, bytes,
-                                focal_kv8_decode_counter_bytes((int)B, (int)T, (int)Hq, cache.num_kv_heads));
+    ws_t = capturable_workspace(kWsKv8, q.device(), stream, bytes, focal_kv8_decode_counter_bytes());
     ws = ws_t.data_ptr();
   }
   raise_on(focal_kv8_decode(q.data_ptr(), o.data_ptr(), &cache, block_table.data_ptr<int32_t>(),

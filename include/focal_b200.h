@@ -336,11 +336,11 @@ int focal_kv8_append(const focal_kv8_append_args* args, const focal_kv8_cache* c
  *
  * Workspace: focal_kv8_decode_workspace_size() bytes, 256-byte aligned; its
  * first focal_kv8_decode_counter_bytes() bytes must be zero before the first
- * call, and every call that returns FOCAL_OK leaves them zero again.  Calls that
- * share a workspace must be ordered.  A page id or length out of range sets
+ * call, and every call that returns FOCAL_OK leaves them zero again.  Calls of
+ * any shapes may share a workspace, if they are ordered.  A page id or length out of range sets
  * device status 3 and is clamped (the output is then not meaningful). */
 size_t focal_kv8_decode_workspace_size(int B, int T, int Hq, int Hkv, int max_seq_len, int D);
-size_t focal_kv8_decode_counter_bytes(int B, int T, int Hq, int Hkv);
+size_t focal_kv8_decode_counter_bytes(void);
 
 int focal_kv8_decode(const void* q, void* o, const focal_kv8_cache* cache, const int32_t* block_table,
                      const int32_t* seq_lens, int B, int T, int Hq, int max_pages_per_seq, int max_seq_len,

@@ -571,6 +571,33 @@ def test_streams_have_their_own_workspaces(cuda):
     assert all(torch.equal(o, want) for o in outs)
 
 
+@pytest.mark.parametrize("capture", [False, True])
+def test_shapes_share_a_workspace(cuda, capture):
+    """Many segments cut between CTAs, one long sequence, and the many again: what one call
+    leaves behind in the workspace means nothing to the next."""
+    big, small = [300 - b % 7 * 40 for b in range(64)], [40000]
+    calls, want = [], []
+    for lens, H, seed in ((big, 32, 5), (small, 2, 6)):
+        table, pages = table_for(lens, 64, cuda, seed=seed)
+        cache = random_cache(pages, H, 64, 64, E4M3, cuda, seed=seed)
+        q = torch.randn(len(lens), 8 * H, 64, device=cuda, generator=gen(cuda, seed)).to(BF16)
+        calls.append((q, cache, table, ints(lens, cuda), max(lens)))
+        o, a, s, w = ok.attention(q[:, None], doubles(cache), table.cpu(), lens)
+        want.append((o[:, 0], attention_tolerance((o, a, s, w), BF16, 64)[:, 0]))
+    order = [0, 1, 0, 0, 1, 0]
+    run = lambda: [F.gqa_decode_attention_kv8(*calls[i]) for i in order]  # noqa: E731
+    outs = run()
+    if capture:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = run()
+        for _ in range(2):
+            g.replay()
+    for i, got in zip(order, outs):
+        assert torch.all((got.double() - want[i][0]).abs() <= want[i][1])
+    assert status() == 0
+
+
 def test_cache_past_32_bits(cuda):
     """Pages whose codes lie past 2^32 bytes: written, read, and nothing at the wrapped
     addresses touched."""

@@ -127,9 +127,9 @@ def test_decode_workspace_sizing():
     L = _lib.lib()
     ws, counters = L.focal_kv8_decode_workspace_size, L.focal_kv8_decode_counter_bytes
     assert 0 < ws(1, 1, 32, 8, 512, 128) <= ws(8, 1, 32, 8, 32768, 128)
-    assert counters(1, 1, 32, 8) % 256 == 0 and counters(1, 1, 32, 8) <= ws(1, 1, 32, 8, 1, 128)
+    assert counters() % 256 == 0 and counters() < ws(1, 1, 32, 8, 1, 128)
     for bad in ((0, 1, 32, 8), (1, 0, 32, 8), (1, 17, 32, 8), (1, 1, 30, 8), (1, 1, 32, 1)):
-        assert ws(*bad, 512, 128) == 0 and counters(*bad) == 0
+        assert ws(*bad, 512, 128) == 0
     assert ws(1, 1, 32, 8, 512, 96) == 0 and ws(1, 1, 32, 8, 0, 128) == 0
 
 

@@ -49,7 +49,10 @@ constexpr int kHalfBytes = kTile * 128;        // 64 positions x 64 dims x 2 B
 constexpr int kKVStageBytes = 4 * kHalfBytes;  // K lo/hi + V lo/hi
 constexpr int kMaxGroup = 16;
 constexpr int kMaxSplits = 128;
-constexpr int kCounterBytes = 256;     // counters region granularity
+constexpr int kMaxHeads = 65535;       // B * Hkv
+// The counters' region has the same size for all shapes: calls of different shapes share a
+// workspace, and none may leave its partials where another's counters are.
+constexpr int kCounterBytes = (kMaxHeads + 1) * 4;
 constexpr int kCombineBatch = 8;      // split partials loaded together by the combining CTA
 
 struct Params {
@@ -509,9 +512,8 @@ size_t workspace_size(int B, int Hq, int Hkv, int L) {
   const int tiles = (L + kTile - 1) / kTile;
   const int smax = tiles < kMaxSplits ? tiles : kMaxSplits;
   const int grp = Hq / Hkv;
-  const size_t counters = ((size_t)bhn * 4 + kCounterBytes - 1) / kCounterBytes * kCounterBytes;
   const size_t recs = (size_t)bhn * smax * grp;
-  return counters + recs * kD * 4 + recs * 2 * 4;
+  return kCounterBytes + recs * kD * 4 + recs * 2 * 4;
 }
 
 int check(int B, int Hq, int Hkv, int L, int D) {
@@ -519,7 +521,7 @@ int check(int B, int Hq, int Hkv, int L, int D) {
   if (D != kD) return set_error(FOCAL_ERR_UNSUPPORTED, "unsupported head_dim (must be 128)");
   if (Hq % Hkv != 0) return set_error(FOCAL_ERR_UNSUPPORTED, "Hq must be a multiple of Hkv");
   if (Hq / Hkv > kMaxGroup) return set_error(FOCAL_ERR_UNSUPPORTED, "Hq / Hkv must be <= 16");
-  if ((long long)B * Hkv > 65535) return set_error(FOCAL_ERR_UNSUPPORTED, "B * Hkv too large");
+  if ((long long)B * Hkv > kMaxHeads) return set_error(FOCAL_ERR_UNSUPPORTED, "B * Hkv too large");
   return FOCAL_OK;
 }
 
@@ -538,10 +540,9 @@ int fill_params(Params* pp, const void* q, void* o, int B, int Hq, int Hkv, int 
     if (!workspace || ws_bytes < need)
       return set_error(FOCAL_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need, ws_bytes);
     if (!aligned(workspace, 256)) return set_error(FOCAL_ERR_INVALID_VALUE, "workspace must be 256-byte aligned");
-    const size_t counters = ((size_t)bhn * 4 + kCounterBytes - 1) / kCounterBytes * kCounterBytes;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     p.counters = reinterpret_cast<unsigned int*>(ws);
-    p.part_o = reinterpret_cast<float*>(ws + counters);
+    p.part_o = reinterpret_cast<float*>(ws + kCounterBytes);
     p.part_ml = p.part_o + (size_t)bhn * pl.splits * grp * kD;
   }
   p.status = dev.status;

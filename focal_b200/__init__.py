@@ -316,7 +316,8 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, cache, block_table: torch.Tenso
     none of them more than max_new, a host integer), or without cu_new T / B rows
     each.  They become the last positions of seq_lens[b] (int32 [B]), which counts
     them already; block_table int32 [B, max_pages].  With inv_freq, k is turned by
-    its positions first (see rope) and so is q [T, Hq, D], which is returned.
+    its positions first (see rope) and so is q [T, Hq, D], which is returned (rows that belong to no sequence, behind
+    cu_new[B], are not written).
 
     Every 16 consecutive tokens of a page and head share a scale: e4m3 the
     smallest power of two >= amax / 448, int8 amax / 127.  It grows when later
@@ -352,13 +353,9 @@ def decode_attention_kv8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cach
     """The attention of a decode step behind its QKV projection: q [B * T, Hq, D],
     k and v [B * T, Hkv, D] (T new tokens per sequence, counted by seq_lens
     already) are turned, k and v appended, and the queries attend over the cache.
-    Returns o [B * T, Hq, D]."""
-    turned = kv8_append(k, v, cache, block_table, seq_lens, q=q, inv_freq=inv_freq, interleaved=interleaved,
-                        mscale=mscale)
-    B = seq_lens.shape[0]
-    o = gqa_decode_attention_kv8(turned.view(B, -1, *turned.shape[1:]), cache, block_table, seq_lens, max_seq_len,
-                                 scale)
-    return o.view(turned.shape)
+    Returns o [B * T, Hq, D].  A call that is refused leaves the cache as it was."""
+    return _ext().decode_attention_kv8(q, k, v, *cache, block_table, seq_lens, max_seq_len, inv_freq, interleaved,
+                                       mscale, scale)
 
 
 __all__ = [

@@ -385,7 +385,7 @@ extern "C" int focal_kv8_append(const focal_kv8_append_args* a, const focal_kv8_
     return set_error(FOCAL_ERR_UNSUPPORTED, "token and head strides must be multiples of 16 bytes");
   const long long pieces = ((long long)a->max_new + 30) / kGroup;  // blocks that max_new rows can touch
   if (pieces * a->B > INT32_MAX) return set_error(FOCAL_ERR_UNSUPPORTED, "B * max_new too large");
-  if (a->B == 0 || a->T == 0 || a->max_new == 0) return FOCAL_OK;
+  if (a->B == 0 || a->T == 0) return FOCAL_OK;  // max_new = 0 is launched: cu_new may say otherwise
   rc = check_cache_pointers(cache);
   if (rc) return rc;
   if (!a->k || !a->v || !a->block_table || !a->seq_lens || (a->rot && !a->inv_freq) || (a->Hq && (!a->q || !a->q_out)))

@@ -905,6 +905,7 @@ int row_chunks(int T, int Hq, int Hkv) { return (T * (Hq / Hkv) + kRowsPerCta - 
 int check_decode(int B, int T, int Hq, int Hkv, int max_seq_len, int D) {
   if (B < 1 || Hq < 1 || Hkv < 1 || max_seq_len < 1)
     return set_error(FOCAL_ERR_UNSUPPORTED, "B, Hq, Hkv and max_seq_len must be positive");
+  if (max_seq_len > 1 << 30) return set_error(FOCAL_ERR_UNSUPPORTED, "max_seq_len must be at most 2^30");
   if (T < 1 || T > kMaxQueryTokens)
     return set_error(FOCAL_ERR_UNSUPPORTED, "query tokens per sequence must be 1 to %d", kMaxQueryTokens);
   if (D != 64 && D != 128) return set_error(FOCAL_ERR_UNSUPPORTED, "unsupported head_dim (must be 64 or 128)");

@@ -528,6 +528,39 @@ c10::optional<torch::Tensor> kv8_append(torch::Tensor k, torch::Tensor v, torch:
   return turned;
 }
 
+// The checks of kv8_attention; returns its workspace's size.
+size_t check_attention(const torch::Tensor& q, int64_t B, int64_t T, const focal_kv8_cache& cache,
+                       const torch::Tensor& block_table, const torch::Tensor& seq_lens, int64_t max_seq_len,
+                       c10::optional<double> scale) {
+  const int64_t Hq = q.size(-2), D = q.size(-1);
+  check_tables(block_table, seq_lens, B, q);
+  TORCH_CHECK(D == cache.head_dim, "k_pages must have shape [num_pages, Hkv, page_size, D]");
+  TORCH_CHECK(T <= INT32_MAX && Hq <= INT32_MAX && max_seq_len <= INT32_MAX && max_seq_len >= 1, "unsupported size");
+  const size_t bytes =
+      focal_kv8_decode_workspace_size((int)B, (int)T, (int)Hq, cache.num_kv_heads, (int)max_seq_len, (int)D);
+  if (bytes == 0) raise_on(FOCAL_ERR_UNSUPPORTED);
+  TORCH_CHECK(max_seq_len <= block_table.size(1) * cache.page_size, "max_seq_len exceeds max_pages_per_seq * page_size");
+  TORCH_CHECK(!scale.has_value() || ((float)*scale > 0.f && std::isfinite((float)*scale)),
+              "scale must be positive and finite");
+  return bytes;
+}
+
+// q, o [B * T, Hq, D] in any shape that ends so
+torch::Tensor kv8_attention(const torch::Tensor& q, int64_t B, int64_t T, int dtype, const focal_kv8_cache& cache,
+                            const torch::Tensor& block_table, const torch::Tensor& seq_lens, int64_t max_seq_len,
+                            c10::optional<double> scale) {
+  const size_t bytes = check_attention(q, B, T, cache, block_table, seq_lens, max_seq_len, scale);
+  const double sc = scale.has_value() ? *scale : 1.0 / std::sqrt((double)cache.head_dim);
+  const c10::cuda::CUDAGuard guard(q.device());
+  auto o = empty_like_rows(q);
+  const cudaStream_t stream = current_stream();
+  const auto ws = capturable_workspace(kWsKv8, q.device(), stream, bytes, focal_kv8_decode_counter_bytes());
+  raise_on(focal_kv8_decode(q.data_ptr(), o.data_ptr(), &cache, block_table.data_ptr<int32_t>(),
+                            seq_lens.data_ptr<int32_t>(), (int)B, (int)T, (int)q.size(-2), (int)block_table.size(1),
+                            (int)max_seq_len, (float)sc, dtype, ws.data_ptr(), bytes, stream));
+  return o;
+}
+
 torch::Tensor gqa_decode_attention_kv8(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages,
                                        torch::Tensor k_scales, torch::Tensor v_scales, torch::Tensor block_table,
                                        torch::Tensor seq_lens, int64_t max_seq_len, c10::optional<double> scale) {
@@ -536,26 +569,28 @@ torch::Tensor gqa_decode_attention_kv8(torch::Tensor q, torch::Tensor k_pages, t
   const int dtype = dtype_of(q, "q", false);
   TORCH_CHECK(q.dim() == 3 || q.dim() == 4, "q must have shape [B, Hq, D] or [B, T, Hq, D]");
   const focal_kv8_cache cache = kv8_cache_of(k_pages, v_pages, k_scales, v_scales, q, "q");
-  const int64_t B = q.size(0), T = q.dim() == 4 ? q.size(1) : 1, Hq = q.size(-2), D = q.size(-1);
-  check_tables(block_table, seq_lens, B, q);
-  TORCH_CHECK(D == cache.head_dim, "k_pages must have shape [num_pages, Hkv, page_size, D]");
-  TORCH_CHECK(T <= INT32_MAX && Hq <= INT32_MAX && max_seq_len <= INT32_MAX && max_seq_len >= 1, "unsupported size");
-  const double sc = scale.has_value() ? *scale : 1.0 / std::sqrt((double)D);
-  const c10::cuda::CUDAGuard guard(q.device());
-  auto o = empty_like_rows(q);
-  const cudaStream_t stream = current_stream();
-  const size_t bytes =
-      focal_kv8_decode_workspace_size((int)B, (int)T, (int)Hq, cache.num_kv_heads, (int)max_seq_len, (int)D);
-  void* ws = nullptr;
-  torch::Tensor ws_t;
-  if (bytes > 0) {
-    ws_t = capturable_workspace(kWsKv8, q.device(), stream, bytes, focal_kv8_decode_counter_bytes());
-    ws = ws_t.data_ptr();
-  }
-  raise_on(focal_kv8_decode(q.data_ptr(), o.data_ptr(), &cache, block_table.data_ptr<int32_t>(),
-                            seq_lens.data_ptr<int32_t>(), (int)B, (int)T, (int)Hq, (int)block_table.size(1),
-                            (int)max_seq_len, (float)sc, dtype, ws, bytes, stream));
-  return o;
+  return kv8_attention(q, q.size(0), q.dim() == 4 ? q.size(1) : 1, dtype, cache, block_table, seq_lens, max_seq_len,
+                       scale);
+}
+
+// A decode step's append and attention.  What the attention would refuse is
+// refused before the append writes to the cache.
+torch::Tensor decode_attention_kv8(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor k_pages,
+                                   torch::Tensor v_pages, torch::Tensor k_scales, torch::Tensor v_scales,
+                                   torch::Tensor block_table, torch::Tensor seq_lens, int64_t max_seq_len,
+                                   torch::Tensor inv_freq, bool interleaved, double mscale,
+                                   c10::optional<double> scale) {
+  check_rows(k, "k", k);
+  check_rows(q, "q", k);
+  const int dtype = dtype_of(q, "q", false);
+  const focal_kv8_cache cache = kv8_cache_of(k_pages, v_pages, k_scales, v_scales, q, "q");
+  const int64_t B = seq_lens.dim() == 1 ? seq_lens.size(0) : 0;
+  TORCH_CHECK(B > 0 && k.size(0) % B == 0, "every sequence must have the same number of new tokens");
+  const int64_t T = k.size(0) / B;
+  check_attention(q, B, T, cache, block_table, seq_lens, max_seq_len, scale);
+  const auto turned = kv8_append(k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, c10::nullopt, T, q,
+                                 inv_freq, interleaved, mscale);
+  return kv8_attention(*turned, B, T, dtype, cache, block_table, seq_lens, max_seq_len, scale);
 }
 
 }  // namespace
@@ -573,6 +608,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rope", &rope, "rotary positions", pybind11::arg("x"), pybind11::arg("positions"), pybind11::arg("inv_freq"),
         pybind11::arg("interleaved") = false, pybind11::arg("mscale") = 1.0, pybind11::arg("out") = pybind11::none());
   m.def("kv8_append", &kv8_append, "append keys and values to the 8-bit paged KV cache");
+  m.def("decode_attention_kv8", &decode_attention_kv8, "a decode step's append and attention over the 8-bit cache");
   m.def("gqa_decode_attention_kv8", &gqa_decode_attention_kv8, "GQA decode attention over the 8-bit paged KV cache");
   m.def("gqa_decode_attention_paged", &gqa_decode_attention_paged, "paged variable-length GQA decode attention",
         pybind11::arg("q"), pybind11::arg("k_pages"), pybind11::arg("v_pages"), pybind11::arg("block_table"),

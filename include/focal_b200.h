@@ -304,6 +304,8 @@ typedef struct focal_kv8_cache {
  * saturate; NaN becomes e4m3's NaN or int8's 0.  All the rows appended to a page
  * must belong to one sequence of the call.
  *
+ * Rows of q_out that belong to no sequence are not written.
+ *
  * Contract: n <= max_new for every sequence (max_new, on the host, sizes the
  * launch); k, v, q [T, heads, head_dim] of dtype bf16 or fp16 with strides in
  * elements (multiples of 16 bytes), 16-byte aligned; q_out [T, Hq, head_dim]
@@ -332,7 +334,8 @@ int focal_kv8_append(const focal_kv8_append_args* args, const focal_kv8_cache* c
  * must not be negative.  Which tiles are summed together depends on the whole batch's
  * lengths, so a sequence's result may differ in its last bits between batches;
  * equal calls give equal bits.
- * Contract: Hq % num_kv_heads == 0, Hq / num_kv_heads <= 16, 1 <= T <= 16.
+ * Contract: Hq % num_kv_heads == 0, Hq / num_kv_heads <= 16, 1 <= T <= 16,
+ * max_seq_len <= 2^30.
  *
  * Workspace: focal_kv8_decode_workspace_size() bytes, 256-byte aligned; its
  * first focal_kv8_decode_counter_bytes() bytes must be zero before the first

@@ -482,6 +482,44 @@ def test_refusals(cuda):
     assert status() == 0
 
 
+def test_refused_steps_leave_the_cache(cuda):
+    """Whatever the composite refuses, it refuses before the append."""
+    table, pages = table_for([64, 64], 64, cuda, seed=1)
+    cache = random_cache(pages, 2, 64, 128, E4M3, cuda, seed=1)
+    before = clones(cache)
+    f, _ = F.rope_inv_freq(128, device=cuda)
+    rows = lambda n, h: torch.ones(n, h, 128, device=cuda, dtype=BF16)  # noqa: E731
+    lens = ints([40, 41], cuda)
+    for n, h, kw, text in ((2, 7, {}, "multiple of Hkv"), (2, 64, {}, "<= 16"), (34, 8, {}, "query tokens"),
+                           (0, 8, {}, "query tokens"), (3, 8, {}, "same number"), (2, 8, dict(max_len=1000), "max_seq_len"),
+                           (2, 8, dict(max_len=0), "size"), (2, 8, dict(scale=0.0), "scale"),
+                           (2, 8, dict(scale=1e-60), "scale"), (2, 8, dict(scale=float("inf")), "scale"),
+                           (2, 8, dict(mscale=float("nan")), "mscale"), (2, 8, dict(f=f.float()), "dtype"),
+                           (2, 8, dict(q=rows(1, 8)), "shape"), (2, 8, dict(q=rows(2, 8).half()), "dtype")):
+        a = dict(dict(q=rows(n, h), max_len=64, f=f, mscale=1.0, scale=None), **kw)
+        with pytest.raises(RuntimeError, match=text):
+            F.decode_attention_kv8(a["q"], rows(n, 2), rows(n, 2), cache, table, lens, a["max_len"], a["f"],
+                                   mscale=a["mscale"], scale=a["scale"])
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(cache, before))
+    assert status() == 0
+
+
+def test_append_of_more_than_max_new_is_reported(cuda):
+    """cu_new that brings rows where max_new says none: nothing written, and status set."""
+    cache = empty_cache(4, 1, 16, 64, E4M3, cuda)
+    before = clones(cache)
+    x = torch.ones(3, 1, 64, device=cuda, dtype=BF16)
+    args = cache, ints([[0], [1]], cuda), ints([2, 1], cuda)
+    F.kv8_append(x, x, *args, cu_new=ints([0, 0, 0], cuda), max_new=0)
+    torch.cuda.synchronize()
+    assert status() == 0
+    F.kv8_append(x, x, *args, cu_new=ints([0, 2, 3], cuda), max_new=0)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="bad paged-KV index"):
+        F.kv8_append(x, x, *args, cu_new=ints([0, 2, 3], cuda), max_new=2)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, before))
+
+
 # ---------------------------------------------------------- used together
 def decode_run(cuda, code, interleaved, steps, T, prompt, capture=False):
     """A prompt and decode steps of T tokens through the composite, as a server would

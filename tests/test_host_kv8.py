@@ -85,6 +85,7 @@ def test_append_refusals():
     refused(append(k=FAKE + 2), V, "aligned")
     refused(append(cache(k_pages=None)), V, "null")
     refused(append(cache(v_scales=FAKE + 4)), V, "aligned")
+    refused(append(cu_new=FAKE + 2, max_new=0), V, "aligned")
     assert append(T=0, B=0, max_new=0, k=None) == _lib.FOCAL_OK
     L = _lib.lib()
     refused(L.focal_kv8_append(None, ctypes.byref(cache()), None), V, "null")
@@ -110,6 +111,7 @@ def test_decode_refusals():
     refused(decode(B=40000), U, "too large")
     refused(decode(max_len=129), U, "max_seq_len exceeds")
     refused(decode(max_len=0), U, "positive")
+    refused(decode(max_len=(1 << 30) + 1, max_pages=1 << 30), U, "2^30")
     refused(decode(dtype=_lib.FOCAL_FP32), U, "dtype")
     refused(decode(scale=0.0), V, "scale")
     refused(decode(scale=float("nan")), V, "scale")
@@ -154,3 +156,5 @@ def test_python_refusals():
         F.rope(k, torch.arange(3), torch.ones(64).double())
     with pytest.raises(RuntimeError, match="CUDA tensor"):
         F.gqa_decode_attention_kv8(k, c, table, lens, 32)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        F.decode_attention_kv8(k[:2], k[:2], k[:2], c, table, lens, 32, torch.ones(64).double())

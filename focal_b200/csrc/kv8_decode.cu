@@ -68,7 +68,7 @@ constexpr int kMaxCtas = 256;
 // same first one.  So the counters lie in the same place for calls of all shapes, and stay
 // zero between calls that share a workspace.
 constexpr int kCounterBytes = kMaxCtas * 4;
-constexpr int kBatch = 16;  // records whose loads a join has in flight
+constexpr int kBatch = 16;  // records' rows whose loads a warp of a join has in flight
 constexpr int kJoin = 4;    // ways that many records are shared out
 constexpr float kWeightUp = 32768.f;
 
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(32 * warps_of(D))
   // kHbm for each of all tiles, a CTA kOwn for each of its own (measured with 128
   // CTAs at work), a join and what goes with it 2000 and 3500.
   constexpr float kHbm = D == 128 ? 4.8f : 2.4f;
-  constexpr float kOwn = (D == 128 ? 520.f : 330.f) * (NT == 2 ? 1.25f : 1.f) * (INT8 ? 1.2f : 1.f);
+  constexpr float kOwn = (D == 128 ? 520.f : 330.f) * (INT8 ? 1.2f : 1.f);
   const int cta = blockIdx.x;
   int ways = p.ways, per = p.per;
   int total = 0, len32 = 0;
@@ -816,58 +816,75 @@ __global__ void __launch_bounds__(32 * warps_of(D))
     const int row0 = (s2 - kvh * p.chunks) * kRowsPerCta, rows = min(kRowsPerCta, p.T * p.grp - row0);
     int c0;
     const int n = ctas_of(seg, c0);
-    // A warp takes a row and, of many records, every kJoin-th; a lane has kLane dims of it.
-    const int ways = n > kBatch ? kJoin : 1;
-    for (int task = part && last[0] ? (warp + kWarps - rows % kWarps) % kWarps : warp; task < rows * ways; task += kWarps) {
-      const int row = ways == 1 ? task : task / kJoin, way = ways == 1 ? 0 : task % kJoin;
-      float mu = -INFINITY, l = 0.f;
-      float a[kLane];
+    // A warp takes NT rows (two of 16: with one, a CTA that joined two segments took four turns)
+    // and, of many records, every kJoin-th; a lane has kLane dims of them.
+    constexpr int kRecords = kBatch / NT;  // of a row, whose loads are in flight together
+    const int ways = n > kRecords ? kJoin : 1, units = (rows + NT - 1) / NT;
+    for (int task = part && last[0] ? (warp + kWarps - units % kWarps) % kWarps : warp; task < units * ways; task += kWarps) {
+      const int unit = ways == 1 ? task : task / kJoin, way = ways == 1 ? 0 : task % kJoin;
+      float mu[NT], l[NT], a[NT][kLane];
 #pragma unroll
-      for (int i = 0; i < kLane; ++i) a[i] = 0.f;
-      for (int s0 = way; s0 < n; s0 += kBatch * ways) {
-        float2 ml[kBatch];
-        float v[kBatch][kLane];
+      for (int k = 0; k < NT; ++k) {
+        mu[k] = -INFINITY;
+        l[k] = 0.f;
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          const int at = s0 + u * ways;
-          ml[u] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-          for (int i = 0; i < kLane; ++i) v[u][i] = 0.f;
-          if (at < n) {  // the segment's first CTA has it as its last, the others as their first
-            const float* rec = p.cta_rec + (size_t)(2 * (c0 + at) + (at == 0)) * kRec;
-            ml[u] = __ldcg(reinterpret_cast<const float2*>(rec + kRows * kRow + 2 * row));
-            const LaneVec x = __ldcg(reinterpret_cast<const LaneVec*>(rec + row * kRow) + lane);
-            memcpy(v[u], &x, sizeof(x));
-          }
-        }
-        float nm = mu;
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) nm = fmaxf(nm, ml[u].x);
-        const float ref = nm == -INFINITY ? 0.f : nm;
-        const float r = exp2_fast(mu - ref);
-        l *= r;
-#pragma unroll
-        for (int i = 0; i < kLane; ++i) a[i] *= r;
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          const float wgt = exp2_fast(ml[u].x - ref);
-          l += wgt * ml[u].y;
-#pragma unroll
-          for (int i = 0; i < kLane; ++i) a[i] += wgt * v[u][i];
-        }
-        mu = nm;
+        for (int i = 0; i < kLane; ++i) a[k][i] = 0.f;
       }
-      if (ways == 1) {
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll 1
+      for (int s0 = way; s0 < n; s0 += kRecords * ways) {
+        float2 ml[NT][kRecords];
+        float v[NT][kRecords][kLane];
 #pragma unroll
-        for (int i = 0; i < kLane; i += 2)
-          *reinterpret_cast<uint32_t*>(o + row_at(b, kvh, row0 + row) + lane * kLane + i) = pack2<T>(a[i] * inv, a[i + 1] * inv);
-      } else {  // over the rings, which have been read
-        float* rec = reinterpret_cast<float*>(sm) + (size_t)task * (D + 4);
-        LaneVec x;
-        memcpy(&x, a, sizeof(x));
-        reinterpret_cast<LaneVec*>(rec)[lane] = x;
-        if (lane == 0) *reinterpret_cast<float2*>(rec + D) = make_float2(mu, l);
+        for (int k = 0; k < NT; ++k)
+#pragma unroll
+          for (int u = 0; u < kRecords; ++u) {
+            const int at = s0 + u * ways, row = unit * NT + k;
+            ml[k][u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int i = 0; i < kLane; ++i) v[k][u][i] = 0.f;
+            if (at < n && (NT == 1 || row < rows)) {  // the segment's first CTA has it as its last, the others as their first
+              const float* rec = p.cta_rec + (size_t)(2 * (c0 + at) + (at == 0)) * kRec;
+              ml[k][u] = __ldcg(reinterpret_cast<const float2*>(rec + kRows * kRow + 2 * row));
+              const LaneVec x = __ldcg(reinterpret_cast<const LaneVec*>(rec + row * kRow) + lane);
+              memcpy(v[k][u], &x, sizeof(x));
+            }
+          }
+#pragma unroll
+        for (int k = 0; k < NT; ++k) {
+          float nm = mu[k];
+#pragma unroll
+          for (int u = 0; u < kRecords; ++u) nm = fmaxf(nm, ml[k][u].x);
+          const float ref = nm == -INFINITY ? 0.f : nm;
+          const float r = exp2_fast(mu[k] - ref);
+          l[k] *= r;
+#pragma unroll
+          for (int i = 0; i < kLane; ++i) a[k][i] *= r;
+#pragma unroll
+          for (int u = 0; u < kRecords; ++u) {
+            const float wgt = exp2_fast(ml[k][u].x - ref);
+            l[k] += wgt * ml[k][u].y;
+#pragma unroll
+            for (int i = 0; i < kLane; ++i) a[k][i] += wgt * v[k][u][i];
+          }
+          mu[k] = nm;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        const int row = unit * NT + k;
+        if (NT > 1 && row >= rows) break;
+        if (ways == 1) {
+          const float inv = l[k] == 0.f ? 0.f : 1.0f / l[k];
+#pragma unroll
+          for (int i = 0; i < kLane; i += 2)
+            *reinterpret_cast<uint32_t*>(o + row_at(b, kvh, row0 + row) + lane * kLane + i) = pack2<T>(a[k][i] * inv, a[k][i + 1] * inv);
+        } else {  // over the rings, which have been read
+          float* rec = reinterpret_cast<float*>(sm) + (size_t)(row * kJoin + way) * (D + 4);
+          LaneVec x;
+          memcpy(&x, a[k], sizeof(x));
+          reinterpret_cast<LaneVec*>(rec)[lane] = x;
+          if (lane == 0) *reinterpret_cast<float2*>(rec + D) = make_float2(mu[k], l[k]);
+        }
       }
     }
     if (ways > 1) {

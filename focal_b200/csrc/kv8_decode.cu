@@ -39,10 +39,14 @@
 //  * A weight enters P V as f16(2^15 p vs / R): 2^15 moves it up in f16's range
 //    (p >= 2^-29 keeps f16's 11 bits), vs is its block's V scale and R the smallest power
 //    of two >= the V scales seen by the warp so far, so vs / R <= 1; when R
-//    grows the accumulators are rescaled as they are when the maximum grows.
+//    grows the accumulators are rescaled as they are when the maximum grows.  For fp16
+//    outputs it enters as two numbers, that and f16 of the rest: rounding the weights once
+//    is off by as much as rounding the output (together 1.4 times it, up to 2.6 times for a
+//    sequence of one; 16 ragged sequences 21.7 -> 22.5 us, 8 of up to 8191 with 4 tokens
+//    27.9 -> 30.7).  For bf16 outputs it is an eighth of that.
 // What is left: launch, lengths, page ids and the first tiles one after another
 // (about 4 us), and merge and join at the end (1 to 3 us); one sequence of 512
-// takes 5.8 us, 16 ragged ones of up to 4096 21.9 where their bytes take 11.4.
+// takes 5.8 us, 16 ragged ones of up to 4096 21.7 where their bytes take 11.4.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -154,6 +158,7 @@ __global__ void __launch_bounds__(32 * warps_of(D))
   constexpr int kRows = 8 * NT;
   constexpr int kRow = S::kRow;
   constexpr int kLane = D / 32;
+  constexpr int kTerms = std::is_same<T, __half>::value ? 2 : 1;  // f16 numbers that a weight enters P V as
   using LaneVec = typename std::conditional<D == 128, float4, float2>::type;
   constexpr int kRec = kRows * (kRow + 2);  // floats of a record: [row][kRow], [row]{maximum, sum}
   extern __shared__ uint8_t smem_raw[];
@@ -644,15 +649,20 @@ __global__ void __launch_bounds__(32 * warps_of(D))
 #pragma unroll
     for (int m = 0; m < kBlocks; ++m) {
       const float vm = vs[m] * vinv * kWeightUp;
-      uint32_t pb[NT][2];
+      uint32_t pb[NT][kTerms][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const float e0 = exp2_fast(s[m][n][0] - mref[n][0]), e1 = exp2_fast(s[m][n][1] - mref[n][1]);
         const float e2 = exp2_fast(s[m][n][2] - mref[n][0]), e3 = exp2_fast(s[m][n][3] - mref[n][1]);
         lrow[n][0] += e0 + e2;
         lrow[n][1] += e1 + e3;
-        pb[n][0] = movmatrix_trans(pack2<__half>(e0 * vm, e1 * vm));
-        pb[n][1] = movmatrix_trans(pack2<__half>(e2 * vm, e3 * vm));
+        const float w[4] = {e0 * vm, e1 * vm, e2 * vm, e3 * vm};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t hi = pack2<__half>(w[2 * i], w[2 * i + 1]);
+          pb[n][0][i] = movmatrix_trans(hi);
+          if (kTerms == 2) pb[n][kTerms - 1][i] = movmatrix_trans(pack2<__half>(w[2 * i] - half_lo(hi), w[2 * i + 1] - half_hi(hi)));
+        }
       }
       const int vrow = 16 * m + 8 * (lm & 1) + lr;
 #pragma unroll
@@ -662,11 +672,15 @@ __global__ void __launch_bounds__(32 * warps_of(D))
         codes_to_f16<INT8, true>(r0, a0, a1);
         codes_to_f16<INT8, true>(r1, a2, a3);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16_16816(acc[c][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int k = 0; k < kTerms; ++k) mma_f16_16816(acc[c][n], a0, a1, a2, a3, pb[n][k][0], pb[n][k][1]);
         codes_to_f16<INT8, true>(r2, a0, a1);
         codes_to_f16<INT8, true>(r3, a2, a3);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16_16816(acc[c + 1][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int k = 0; k < kTerms; ++k) mma_f16_16816(acc[c + 1][n], a0, a1, a2, a3, pb[n][k][0], pb[n][k][1]);
       }
     }
     fence_proxy_async_smem();  // our reads and zeros of V's slot precede its refill, the K after next

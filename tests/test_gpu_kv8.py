@@ -274,14 +274,16 @@ def test_append_refusals_on_the_device(cuda):
 def attention_tolerance(bounds, dtype, D):
     """`bounds` as ok.attention gives them.  Scores: D products and sums and a handful of
     scalings in fp32, (D + 16) 2^-24 of scale * sum |q| |k| at most; a weight is off by
-    twice that (numerator and sum), by half a step of the 16-bit weight (2^-11) and by
+    twice that (numerator and sum), by half a step of the 16-bit weight (2^-11; 2^-22 for fp16,
+    whose weights are two 16-bit numbers, the second the rounding of the first) and by
     the fp32 exponentials and sums, 2^-18; what a weight's error moves is at most its
     share of sum p |v|.  A weight enters as f16(2^15 p vs / R) with R at most twice the
     largest V scale: below f16's normal numbers that is off by up to 2^-25, which is
     2^-40 R / vs of the weight of the maximum, so 2^-39 times the largest V scale and
     code for each position.  Then the output's rounding (and fp16's smallest subnormal's half)."""
     o, a, s, w = bounds
-    noise = (2 * (D + 16) * 2.0 ** -24 * s + 2.0 ** -11 + 2.0 ** -18) * a + 2.0 ** -39 * w
+    weight = 2.0 ** -22 if dtype == FP16 else 2.0 ** -11
+    noise = (2 * (D + 16) * 2.0 ** -24 * s + weight + 2.0 ** -18) * a + 2.0 ** -39 * w
     return noise + (o.abs() + noise) * (torch.finfo(dtype).eps / 2) + 2.0 ** -25 * (dtype == FP16)
 
 

@@ -26,8 +26,8 @@
 // turning it on by inv_freq in 64 bits.
 //
 // Bound: HBM and the issue of some 800 instructions a job for prompts (8 x 1024
-// tokens of 32 + 16 heads 34.2 us, 0.83 of the measured copy rate; 5072 tokens in
-// five prompts 22.8 us, 0.77), the chain of dependent loads (length, then page and
+// tokens of 32 + 16 heads 34.0 us, 0.83 of the measured copy rate; 5072 tokens in
+// five prompts 22.7 us, 0.77), the chain of dependent loads (length, then page and
 // rows) for a step (8 tokens 3.5 us), whose heads are spread over thread blocks.
 // Measured against it: the 64 values of a lane held in registers between
 // the two passes, 8 warps a thread block, two blocks an SM: 38.4 and 30.3 us.
@@ -265,24 +265,22 @@ __global__ void __launch_bounds__(32 * kAppendWarps, kBlocksPerSm) append_kernel
     // Twice over the rows, for amax and for the codes: turning them again costs less than
     // the registers that would hold them.  Infinities saturate and NaN is stored as NaN
     // (e4m3) or 0 (int8); neither sets the scale.
-    float amax = 0.f;
-#pragma unroll 1
-    for (int finite = 0; finite < 2; ++finite) {
+    auto amax_of = [&](auto finite) {  // of all values (but NaN), or of the finite ones
+      float amax = 0.f;
 #pragma unroll 1
       for (int i = r0 / kRows; i * kRows < r1; ++i) {
         const int r = i * kRows + rr;
         values(i, val);
         float m = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          if (finite && !(fabsf(val[e]) < INFINITY)) val[e] = 0.f;
-          m = fmaxf(m, fabsf(val[e]));  // not NaN
-        }
+        for (int e = 0; e < 16; ++e)
+          if (!decltype(finite)::value || fabsf(val[e]) < INFINITY) m = fmaxf(m, fabsf(val[e]));
         if (r >= r0 && r < r1) amax = fmaxf(amax, m);
       }
-      if (!__any_sync(0xffffffffu, amax == INFINITY)) break;
-      amax = 0.f;
-    }
+      return amax;
+    };
+    float amax = amax_of(std::false_type());
+    if (__any_sync(0xffffffffu, amax == INFINITY)) amax = amax_of(std::true_type());
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     uint8_t* out = (is_v ? p.v_pages : p.k_pages) + (ph * p.page_size + sub) * D;

@@ -51,7 +51,9 @@ struct AppendParams {
   const double* inv_freq;
   int* status;
   long long kt, kh, vt, vh, qt, qh;  // strides in elements
-  int T, max_new, Hq, Hkv, half, num_pages, page_size, max_pages, pieces, jobs_per_block;
+  int B, T, max_new, Hq, Hkv, half, num_pages, page_size, max_pages;
+  int pieces;  // thread blocks of a sequence; 0: they are shared out by cu_new
+  int jobs_per_block;
   double mscale;
 };
 
@@ -121,7 +123,26 @@ __device__ __forceinline__ void dequantise4(uint32_t c, float (&x)[4]) {
   }
 }
 
-template <typename T, int D, bool INT8, bool INTERLEAVED>
+// The sequence and the piece of its rows that this thread block has, where thread blocks are
+// shared out by cu_new: sequence b's from cu_new[b] / 16 + 2 b on (its n rows touch at most
+// (n + 30) / 16 blocks of the cache, no more than n / 16 + 2).  Every warp looks for itself.
+__device__ __forceinline__ int2 find_block(const int32_t* cu_new, int B, int T, int max_new, int* status) {
+  int found = -1, piece = 0;
+#pragma unroll 1
+  for (int i = threadIdx.x & 31; i < B; i += 32) {
+    const int c0 = cu_new[i], c1 = cu_new[i + 1], at = static_cast<int>(blockIdx.x) - (c0 / kGroup + 2 * i);
+    if (c0 < 0 || c1 > T || c1 < c0 || c1 - c0 > max_new)
+      set_status(status, kDevBadIndex);
+    else if (at >= 0 && at < c1 / kGroup + 2 - c0 / kGroup) {
+      found = i;
+      piece = at;
+    }
+  }
+  const int b = __reduce_max_sync(0xffffffffu, found);
+  return make_int2(b, __shfl_sync(0xffffffffu, piece, b & 31));
+}
+
+template <typename T, int D, bool INT8, bool INTERLEAVED, bool BY_CU>
 __global__ void __launch_bounds__(32 * kAppendWarps, kBlocksPerSm) append_kernel(const AppendParams p) {
   constexpr int kLanes = D / 16;      // lanes of one row
   constexpr int kRows = 32 / kLanes;  // rows that a warp holds side by side
@@ -133,7 +154,16 @@ __global__ void __launch_bounds__(32 * kAppendWarps, kBlocksPerSm) append_kernel
   griddep_launch_dependents();
   griddep_wait();
 
-  const int b = blockIdx.x / p.pieces;
+  int b, piece;
+  if constexpr (!BY_CU) {
+    b = blockIdx.x / p.pieces;
+    piece = blockIdx.x % p.pieces;
+  } else {
+    const int2 at = find_block(p.cu_new, p.B, p.T, p.max_new, p.status);
+    b = at.x;
+    piece = at.y;
+    if (b < 0) return;
+  }
   const int len = p.seq_lens[b];
   const int c0 = p.cu_new ? p.cu_new[b] : b * p.max_new;
   const int c1 = p.cu_new ? p.cu_new[b + 1] : c0 + p.max_new;
@@ -143,7 +173,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps, kBlocksPerSm) append_kernel
     return;
   }
   const int start = len - n;  // position of the first new row
-  const long long at0 = ((long long)(start / kGroup) + blockIdx.x % p.pieces) * kGroup;
+  const long long at0 = ((long long)(start / kGroup) + piece) * kGroup;
   if (n == 0 || at0 >= len) return;
   const int at = static_cast<int>(at0);  // position of the block's row 0
   const int r0 = max(start - at, 0), r1 = min(len - at, kGroup);  // the new rows of the block
@@ -338,21 +368,27 @@ int check_cache_pointers(const focal_kv8_cache* c) {
   return FOCAL_OK;
 }
 
-template <typename T, int D, bool INT8, bool INTERLEAVED>
+template <typename T, int D, bool INT8, bool INTERLEAVED, bool BY_CU>
 int launch_one(const AppendParams& p, int slot, dim3 grid, cudaStream_t s) {
   constexpr int kBytes = kGroup * (D / 2) * 8 + kAppendWarps * 2 * kGroup * D * 2;  // cos and sin, double buffers
-  auto kern = append_kernel<T, D, INT8, INTERLEAVED>;
+  auto kern = append_kernel<T, D, INT8, INTERLEAVED, BY_CU>;
   const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), slot, kBytes);
   if (rc) return rc;
   return launch_pdl(kern, grid, 32 * kAppendWarps, kBytes, s, "append_kernel launch", p);
 }
 
+template <typename T, int D, bool INT8, bool INTERLEAVED>
+int launch_by(const AppendParams& p, int slot, dim3 grid, cudaStream_t s) {
+  return p.pieces ? launch_one<T, D, INT8, INTERLEAVED, false>(p, slot, grid, s)
+                  : launch_one<T, D, INT8, INTERLEAVED, true>(p, slot + 16, grid, s);
+}
+
 template <typename T, int D>
 int launch_append(const AppendParams& p, int code, bool interleaved, int slot, dim3 grid, cudaStream_t s) {
   if (code == FOCAL_INT8)
-    return interleaved ? launch_one<T, D, true, true>(p, slot, grid, s) : launch_one<T, D, true, false>(p, slot + 1, grid, s);
-  return interleaved ? launch_one<T, D, false, true>(p, slot + 2, grid, s)
-                     : launch_one<T, D, false, false>(p, slot + 3, grid, s);
+    return interleaved ? launch_by<T, D, true, true>(p, slot, grid, s) : launch_by<T, D, true, false>(p, slot + 1, grid, s);
+  return interleaved ? launch_by<T, D, false, true>(p, slot + 2, grid, s)
+                     : launch_by<T, D, false, false>(p, slot + 3, grid, s);
 }
 
 }  // namespace kv8
@@ -414,6 +450,7 @@ extern "C" int focal_kv8_append(const focal_kv8_append_args* a, const focal_kv8_
   p.vh = a->v_head_stride;
   p.qt = a->q_token_stride;
   p.qh = a->q_head_stride;
+  p.B = a->B;
   p.T = a->T;
   p.max_new = a->max_new;
   p.Hq = a->Hq;
@@ -422,7 +459,6 @@ extern "C" int focal_kv8_append(const focal_kv8_append_args* a, const focal_kv8_
   p.num_pages = cache->num_pages;
   p.page_size = cache->page_size;
   p.max_pages = a->max_pages_per_seq;
-  p.pieces = static_cast<int>(pieces);
   p.mscale = a->mscale;
   // Heads of a block of tokens are spread over thread blocks until these are
   // eight to an SM (every one of them computes cos and sin anew).
@@ -431,7 +467,12 @@ extern "C" int focal_kv8_append(const focal_kv8_append_args* a, const focal_kv8_
   const int spread = (int)std::min<long long>((jobs + kAppendWarps - 1) / kAppendWarps,
                                               std::max<long long>(1, (8LL * dev.sm_count + blocks - 1) / blocks));
   p.jobs_per_block = ((jobs + spread - 1) / spread + kAppendWarps - 1) / kAppendWarps * kAppendWarps;
-  const dim3 grid(static_cast<unsigned>(pieces * a->B), (jobs + p.jobs_per_block - 1) / p.jobs_per_block, 1);
+  // Each sequence gets as many thread blocks as the longest, most of them without rows where few
+  // are long; beyond eight times as many as needed they are shared out by cu_new (8192 new tokens
+  // beside 127 times one: 158 us and 37; 16 prompts of 5 to 560, twice as many as needed: 21.0 and 21.7).
+  const long long flat = (long long)a->T / kGroup + 2LL * a->B;
+  p.pieces = a->cu_new && 8 * flat < pieces * a->B ? 0 : static_cast<int>(pieces);
+  const dim3 grid(static_cast<unsigned>(p.pieces ? pieces * a->B : flat), (jobs + p.jobs_per_block - 1) / p.jobs_per_block, 1);
   const bool il = a->interleaved != 0;
   if (a->dtype == FOCAL_BF16)
     return D == 128 ? launch_append<__nv_bfloat16, 128>(p, cache->code, il, 60, grid, stream)

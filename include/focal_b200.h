@@ -311,7 +311,8 @@ typedef struct focal_kv8_cache {
  * elements (multiples of 16 bytes), 16-byte aligned; q_out [T, Hq, head_dim]
  * contiguous; rot 0 or a multiple of 16 up to head_dim; Hq = 0 without q.
  * A length, cu_new entry or page id out of range sets device status 3, and
- * nothing is written for that sequence (or block), its rows of q_out among it. */
+ * nothing is written for that sequence (or block), its rows of q_out among it;
+ * beside a cu_new entry out of order, neighbours' rows may be left out too. */
 typedef struct focal_kv8_append_args {
   const void *k, *v, *q;
   void* q_out;

@@ -227,6 +227,41 @@ def test_append_turned(cuda, code, interleaved, D, rot, Hq, H):
     assert status() == 0
 
 
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("new", [[700] + [1] * 40, [1] * 33 + [0, 900, 0, 17] + [2] * 30, [0] * 70 + [333]])
+def test_append_one_long_among_many(cuda, code, new):
+    """Thread blocks shared out by cu_new: the same bits as each sequence appended by itself,
+    and a bad entry among them is reported."""
+    H, D, S, Hq = 2, 128, 32, 4
+    lens = [n + (b * 7) % 45 for b, n in enumerate(new)]
+    table, pages = table_for(lens, S, cuda, seed=9)
+    x = torch.randn(sum(new), Hq + 2 * H, D, device=cuda, generator=gen(cuda, 5)).to(BF16)
+    q, k, v = x[:, :Hq], x[:, Hq:Hq + H], x[:, Hq + H:]
+    f, m = F.rope_inv_freq(D, device=cuda)
+    got, one = random_cache(pages, H, S, D, code, cuda, 9), random_cache(pages, H, S, D, code, cuda, 9)
+    cu = [sum(new[:b]) for b in range(len(new) + 1)]
+    turned = F.kv8_append(k, v, got, table, ints(lens, cuda), cu_new=ints(cu, cuda), max_new=max(new), q=q, inv_freq=f)
+    for b, n in enumerate(new):
+        if n:
+            rows = slice(cu[b], cu[b + 1])
+            alone = F.kv8_append(k[rows], v[rows], one, table[b:b + 1], ints([lens[b]], cuda), q=q[rows], inv_freq=f)
+            assert torch.equal(alone, turned[rows])
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, one))
+    assert status() == 0
+    at = len(new) // 2
+    for bad in (-1, sum(new) + 1):
+        before = clones(got)
+        F.kv8_append(k, v, got, table, ints(lens, cuda), cu_new=ints(cu[:at] + [bad] + cu[at + 1:], cuda), max_new=max(new),
+                     inv_freq=f)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="bad paged-KV index"):
+            F.kv8_append(k, v, got, table, ints(lens, cuda), cu_new=ints(cu, cuda), max_new=max(new), inv_freq=f)
+        for t, u in zip(got, before):  # nothing of the sequences on both sides of it
+            for b in (at - 1, at):
+                own = table[b, :-(-lens[b] // S)].long()
+                assert torch.equal(t[own].view(torch.uint8), u[own].view(torch.uint8))
+
+
 def test_append_steps_equal_a_prompt(cuda):
     """e4m3: one token at a time gives the prompt's scales, and its codes wherever no
     older code sank below the smallest subnormal when it moved."""

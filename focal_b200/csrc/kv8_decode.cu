@@ -193,17 +193,14 @@ __global__ void __launch_bounds__(32 * warps_of(D))
   const int hc = p.Hkv * p.chunks;  // segments of a sequence
   auto tiles_of = [](int len) { return (len + kTile - 1) / kTile; };
   auto len_of = [&](int b) { return min(max(p.seq_lens[b], 0), p.max_len); };
-  auto checked_len = [&](int b) {  // 0 behind the last sequence
-    int n = 0;
-    if (b < p.B) {
-      n = p.seq_lens[b];
-      if (n < 0 || n > p.max_len) {
-        set_status(p.status, kDevBadIndex);
-        n = n < 0 ? 0 : p.max_len;
-      }
+  auto checked = [&](int n) {
+    if (n < 0 || n > p.max_len) {
+      set_status(p.status, kDevBadIndex);
+      n = n < 0 ? 0 : p.max_len;
     }
     return n;
   };
+  auto checked_len = [&](int b) { return b < p.B ? checked(p.seq_lens[b]) : 0; };  // 0 behind the last sequence
 
   // ---- this CTA's tiles: f0 .. f1 - 1 of the flat order.
   // By segments, every CTA has one segment's part (f counts within its sequence):
@@ -222,11 +219,19 @@ __global__ void __launch_bounds__(32 * warps_of(D))
     empty = lane < p.B && len32 == 0;
     int top = tiles_of(len32);  // tiles of one segment of the longest sequence
     total = top;
-    for (int b = lane + 32; b < p.B; b += 32) {
-      const int n = checked_len(b);
-      empty |= n == 0;
-      total += tiles_of(n);
-      top = max(top, tiles_of(n));
+    constexpr int kLens = 8;  // on their way together
+    for (int b0 = lane + 32; b0 - lane < p.B; b0 += 32 * kLens) {
+      int n[kLens];
+#pragma unroll
+      for (int i = 0; i < kLens; ++i) n[i] = b0 + 32 * i < p.B ? p.seq_lens[b0 + 32 * i] : -1;
+#pragma unroll
+      for (int i = 0; i < kLens; ++i) {
+        if (b0 + 32 * i >= p.B) break;
+        n[i] = checked(n[i]);
+        empty |= n[i] == 0;
+        total += tiles_of(n[i]);
+        top = max(top, tiles_of(n[i]));
+      }
     }
     empty = __any_sync(0xffffffffu, empty);
     total = __reduce_add_sync(0xffffffffu, total) * hc;
@@ -294,23 +299,25 @@ __global__ void __launch_bounds__(32 * warps_of(D))
     const int at = p.by_hc(g0);  // in the tiles of one segment of each sequence
     int sum = 0, b0 = 0, n = len32;
     while (true) {
+      const int next = b0 + 32 + lane < p.B ? len_of(b0 + 32 + lane) : 0;
+      const int of32 = __reduce_add_sync(0xffffffffu, tiles_of(n));
+      if (sum + of32 <= at) {
+        sum += of32;
+        b0 += 32;
+        n = next;
+        continue;
+      }
       int incl = tiles_of(n);
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, incl, x);
         if (lane >= x) incl += y;
       }
-      const unsigned int found = __ballot_sync(0xffffffffu, sum + incl > at);
-      if (found) {
-        const int src = __ffs(found) - 1;
-        cb = b0 + src;
-        clen = __shfl_sync(0xffffffffu, n, src);
-        seq_begin = (sum + __shfl_sync(0xffffffffu, incl, src) - tiles_of(clen)) * hc;
-        break;
-      }
-      sum += __shfl_sync(0xffffffffu, incl, 31);
-      b0 += 32;
-      n = b0 + lane < p.B ? len_of(b0 + lane) : 0;
+      const int src = __ffs(__ballot_sync(0xffffffffu, sum + incl > at)) - 1;
+      cb = b0 + src;
+      clen = __shfl_sync(0xffffffffu, n, src);
+      seq_begin = (sum + __shfl_sync(0xffffffffu, incl, src) - tiles_of(clen)) * hc;
+      break;
     }
   }
 

@@ -388,6 +388,27 @@ def test_attention_lengths(cuda, B, L, H, code):
     check_attention(cuda, B, 1, 4 * H, H, 128, 64, lens, L + 100, code, BF16, seed=L)
 
 
+@pytest.mark.parametrize("B,H,top", [(33, 8, 200), (290, 1, 150), (700, 1, 70), (1500, 2, 20)])
+def test_attention_many_sequences(cuda, B, H, top):
+    """More sequences than a warp has lanes, or looks up at once; many of them empty."""
+    g = torch.Generator().manual_seed(B)
+    lens = (torch.randint(-top // 4, top + 1, (B,), generator=g)).clamp(min=0).tolist()
+    got = check_attention(cuda, B, 1, 4 * H, H, 64, 16, lens, top, E4M3, BF16, seed=B)
+    assert got[[n == 0 for n in lens]].count_nonzero() == 0
+    for at in (B - 1, B // 2, 32):
+        bad = list(lens)
+        bad[at] = top + 1
+        table, pages = table_for(lens, 16, cuda, seed=B)
+        table = torch.nn.functional.pad(table, (0, 8), value=0).clamp(min=0).contiguous()
+        cache = random_cache(pages, H, 16, 64, E4M3, cuda, B)
+        q = torch.zeros(B, 4 * H, 64, device=cuda, dtype=BF16)
+        F.gqa_decode_attention_kv8(q, cache, table, ints(bad, cuda), top)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="bad paged-KV index"):
+            F.gqa_decode_attention_kv8(q, cache, table, ints(lens, cuda), top)
+    assert status() == 0
+
+
 def test_attention_peaked_and_flat(cuda):
     """Scores far apart (large q) and all equal (q = 0), large and tiny scales of q."""
     for gain, dtype in ((40.0, BF16), (0.0, BF16), (1e30, BF16), (1e-30, BF16), (2000.0, FP16)):

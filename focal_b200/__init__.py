@@ -274,9 +274,10 @@ def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, inter
     with `interleaved`.
 
     x is bf16, fp16 or fp32 with a contiguous last dimension (a view of packed
-    QKV rows will do); positions int32 or int64 [T]; inv_freq fp64.  Angles, cos
+    QKV rows will do); positions int32 or int64 [T]; inv_freq fp64.  Angles (below 2^50), cos
     and sin are 64-bit, the turn fp32, with one rounding.  Writes a new
-    contiguous tensor, or `out` (x itself works in place).
+    contiguous tensor, or `out` (x itself works in place, any other overlap
+    does not).  For inference: it has no gradient.
     """
     return _ext().rope(x, positions, inv_freq, interleaved, mscale, out)
 

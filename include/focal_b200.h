@@ -262,7 +262,8 @@ int focal_gqa_decode_paged(const void* q, const void* k_pages, const void* v_pag
  *              strides in elements, multiples of 16 bytes; x and y 16-byte
  *              aligned.  y == x with the same strides works in place; other
  *              overlap is not allowed.  x's strides may be 0.
- *   positions  [T] int32, or int64 with positions64; any value
+ *   positions  [T] int32, or int64 with positions64; of either sign, with
+ *              |positions[t] * inv_freq[i]| < 2^50 (beyond it y is meaningless)
  *   inv_freq   fp64 [rot / 2], device memory: radians per position
  * Contract: D % 8 == 0, 16 <= D <= 1024; rot % 16 == 0, 16 <= rot <= D. */
 typedef enum focal_dtype { FOCAL_BF16 = 0, FOCAL_FP16 = 1, FOCAL_FP32 = 2 } focal_dtype;

@@ -89,6 +89,7 @@ SIGNATURES = {
     "focal_kv8_append": (_I, [ctypes.POINTER(Kv8AppendArgs), _K, _P]),
     "focal_kv8_decode_workspace_size": (_S, [_I, _I, _I, _I, _I, _I]),
     "focal_kv8_decode_counter_bytes": (_S, []),
+    "focal_kv8_decode_plan": (_I, [_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_I)]),
     "focal_kv8_decode": (_I, [_P, _P, _K, _P, _P, _I, _I, _I, _I, _I, _F, _I, _P, _S, _P]),
     "focal_device_status": (_I, [ctypes.POINTER(_I)]),
     "focal_device_status_peek": (_I, [ctypes.POINTER(_I)]),

@@ -21,8 +21,13 @@ struct FastDiv {
     while ((1ull << shift) < d) ++shift;
     mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
   }
-  __device__ __forceinline__ int operator()(int n) const {
-    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
+  __host__ __device__ __forceinline__ int operator()(int n) const {
+    const uint32_t u = static_cast<uint32_t>(n);
+#ifdef __CUDA_ARCH__
+    return static_cast<int>((__umulhi(u, mul) + u) >> shift);
+#else
+    return static_cast<int>((static_cast<uint32_t>(static_cast<uint64_t>(u) * mul >> 32) + u) >> shift);
+#endif
   }
 };
 

@@ -76,6 +76,15 @@ constexpr int kBatch = 16;  // records' rows whose loads a warp of a join has in
 constexpr int kJoin = 4;    // ways that many records are shared out
 constexpr float kWeightUp = 32768.f;
 
+// How a call's tiles are shared out, as far as the host knows: `segs` segments of at most
+// `per_seg` tiles on `ctas` CTAs, each segment to `ways` CTAs of `per` tiles (0: more segments than
+// CTAs).  With `decide`, the kernel may share the tiles out evenly instead, or stack `stack`
+// whole segments on a CTA.
+struct Plan {
+  int segs, ways, per, stack, decide, ctas;
+  FastDiv by_ctas, by_ways;
+};
+
 struct DecodeParams {
   const void* q;
   void* o;
@@ -86,13 +95,39 @@ struct DecodeParams {
   unsigned int* counters;  // [CTA]: arrivals at the segment that goes on from it into the next
   int* status;
   int B, T, Hq, Hkv, grp, chunks, num_pages, page_size, max_pages, max_len;
-  // By segments: segs of them, `ways` CTAs each (0: more segments than CTAs) with
-  // `per` tiles each.  With `decide`, the kernel may share the tiles out evenly
-  // instead, or stack `stack` whole segments on a CTA.
-  int segs, ways, per, stack, decide;
+  Plan plan;
   float scale_log2;
-  FastDiv by_hc, by_chunks, by_grp, by_page, by_grid, by_ways;
+  FastDiv by_hc, by_chunks, by_grp, by_page;
 };
+
+// The kernel's decision, for `total` tiles of which the longest segment has `top`: `per` tiles to a
+// CTA, of one segment each (`ways` CTAs a segment), or with `ways` 0 of all tiles in one order.
+// By segments, every CTA has one segment's part: nothing to locate, often nothing to join, but the
+// longest segment sets the time.  In SM cycles: HBM needs kHbm for each of all tiles, a
+// CTA kOwn for each of its own (measured with 128 CTAs at work), a join and what goes with it 2000
+// and 3500.  Every tile has its CTA: per * ways >= top, or per * ctas >= total.
+template <int D, bool INT8>
+__host__ __device__ __forceinline__ void share_out(const Plan& plan, int total, int top, int& ways, int& per) {
+  constexpr float kHbm = D == 128 ? 4.8f : 2.4f;
+  constexpr float kOwn = (D == 128 ? 520.f : 330.f) * (INT8 ? 1.2f : 1.f);
+  const int even = max(4, plan.by_ctas(total + plan.ctas - 1));
+  const float hbm = kHbm * total, evenly = fmaxf(hbm, kOwn * even) + 3500.f;
+  ways = plan.ways;
+  if (ways > 0) {
+    if (top <= warps_of(D) * 3 / 2) ways = 1;
+    const int part = ways == 1 ? top : plan.by_ways(top + ways - 1);
+    per = max(part, 1);
+    if (fmaxf(hbm, kOwn * part) + (ways > 1 ? 2000.f : 0.f) > evenly) {
+      ways = 0;
+      per = even;
+    }
+  } else {
+    per = even;
+    // (the CTAs launched have to hold all segments: a plan that falls short is not taken)
+    if (total == plan.segs * top && (long long)plan.stack * plan.ctas >= plan.segs &&
+        fmaxf(hbm, kOwn * (plan.stack * top)) <= evenly) per = plan.stack * top;
+  }
+}
 
 // A part of a segment: the segment's number (-1: none) and the flat range of all of it.
 struct Portion {
@@ -202,19 +237,12 @@ __global__ void __launch_bounds__(32 * warps_of(D))
   };
   auto checked_len = [&](int b) { return b < p.B ? checked(p.seq_lens[b]) : 0; };  // 0 behind the last sequence
 
-  // ---- this CTA's tiles: f0 .. f1 - 1 of the flat order.
-  // By segments, every CTA has one segment's part (f counts within its sequence):
-  // nothing to locate, often nothing to join, but the longest segment sets the
-  // time.  Evenly, every CTA has `per` tiles of all.  In SM cycles: HBM needs
-  // kHbm for each of all tiles, a CTA kOwn for each of its own (measured with 128
-  // CTAs at work), a join and what goes with it 2000 and 3500.
-  constexpr float kHbm = D == 128 ? 4.8f : 2.4f;
-  constexpr float kOwn = (D == 128 ? 520.f : 330.f) * (INT8 ? 1.2f : 1.f);
+  // ---- this CTA's tiles: f0 .. f1 - 1 of the flat order (by segments, f counts within its sequence)
   const int cta = blockIdx.x;
-  int ways = p.ways, per = p.per;
+  int ways = p.plan.ways, per = p.plan.per;
   int total = 0, len32 = 0;
   bool empty = false;
-  if (p.decide) {
+  if (p.plan.decide) {
     len32 = checked_len(lane);  // the first 32 sequences stay in registers
     empty = lane < p.B && len32 == 0;
     int top = tiles_of(len32);  // tiles of one segment of the longest sequence
@@ -236,23 +264,12 @@ __global__ void __launch_bounds__(32 * warps_of(D))
     empty = __any_sync(0xffffffffu, empty);
     total = __reduce_add_sync(0xffffffffu, total) * hc;
     top = __reduce_max_sync(0xffffffffu, top);
-    const int even = max(4, p.by_grid(total + gridDim.x - 1));
-    const float hbm = kHbm * total, evenly = fmaxf(hbm, kOwn * even) + 3500.f;
-    if (ways > 0) {
-      if (top <= kWarps * 3 / 2) ways = 1;
-      const int part = ways == 1 ? top : p.by_ways(top + ways - 1);
-      per = max(part, 1);
-      if (fmaxf(hbm, kOwn * part) + (ways > 1 ? 2000.f : 0.f) > evenly) ways = 0;
-    } else {
-      per = 0;
-      if (total == p.segs * top && fmaxf(hbm, kOwn * (p.stack * top)) <= evenly) per = p.stack * top;
-    }
-    if (ways == 0 && (p.ways > 0 || per == 0)) per = even;
+    share_out<D, INT8>(p.plan, total, top, ways, per);
   }
   int f0 = 0, f1 = 0, cb = 0, seq_begin = 0, clen = 0, first_cta = 0;
   if (ways > 0) {
-    const int seg = ways == 1 ? cta : p.by_ways(cta);
-    if (seg < p.segs) {
+    const int seg = ways == 1 ? cta : p.plan.by_ways(cta);
+    if (seg < p.plan.segs) {
       first_cta = seg * ways;
       cb = p.by_hc(seg);
       clen = checked_len(cb);
@@ -281,8 +298,8 @@ __global__ void __launch_bounds__(32 * warps_of(D))
   T* o = static_cast<T*>(p.o);
   // sequences without positions have no tiles
   if (ways > 0) {
-    if (clen == 0 && cta == first_cta && cta < p.segs * ways) {
-      const int sl = (ways == 1 ? cta : p.by_ways(cta)) - cb * hc, kvh = p.by_chunks(sl), row0 = (sl - kvh * p.chunks) * kRowsPerCta;
+    if (clen == 0 && cta == first_cta && cta < p.plan.segs * ways) {
+      const int sl = (ways == 1 ? cta : p.plan.by_ways(cta)) - cb * hc, kvh = p.by_chunks(sl), row0 = (sl - kvh * p.chunks) * kRowsPerCta;
       for (int e = threadIdx.x; e < min(kRowsPerCta, p.T * p.grp - row0) * (D / 4); e += kDecodeThreads)
         store4(o + row_at(cb, kvh, row0 + e / (D / 4)) + e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
     }
@@ -953,12 +970,39 @@ int check_decode(int B, int T, int Hq, int Hkv, int max_seq_len, int D) {
   return FOCAL_OK;
 }
 
-// Counters, and records: one per warp and two per CTA.
+Plan plan_for(int segs, int per_seg, int sm_count, int D) {
+  Plan plan{};
+  const int sms = std::min(sm_count, kMaxCtas);
+  const long long tiles = (long long)segs * per_seg;
+  plan.segs = segs;
+  plan.stack = (segs - 1) / sms + 1;
+  plan.ways = sms / segs;
+  if (plan.ways > 0) {
+    // One CTA where its warps have hardly more than a tile each, or else parts of 4 tiles or more; and not so many
+    // that joining them (110 cycles each) costs more than it saves (560 a tile).
+    const int most = (int)(2.25 * std::sqrt((double)per_seg)) + 1;
+    plan.ways = per_seg <= warps_of(D) * 3 / 2 ? 1 : std::min({plan.ways, (per_seg + 3) / 4, most});
+    plan.per = (per_seg + plan.ways - 1) / plan.ways;
+    plan.ways = (per_seg + plan.per - 1) / plan.per;
+    plan.by_ways.set(plan.ways);
+  }
+  // parts this small cannot be uneven enough to matter
+  plan.decide = plan.ways == 0 || plan.per > warps_of(D) * 3 / 2;
+  // More segments than SMs: every SM has a CTA, since the kernel may stack whole segments of one tile on them.
+  plan.ctas = plan.ways == 0 ? sms
+              : plan.decide  ? (int)std::min<long long>(std::max<long long>((tiles + 3) / 4, (long long)segs * plan.ways), sms)
+                             : segs * plan.ways;
+  plan.by_ctas.set(plan.ctas);
+  return plan;
+}
+
+// Counters, and records of 8 or 16 rows: one per warp and two per CTA.
+size_t workspace_of(size_t ctas, int rows, int D) { return kCounterBytes + ctas * (warps_of(D) + 2) * rows * (D + 10) * 4; }
+
 size_t decode_workspace(int B, int T, int Hq, int Hkv, int max_seq_len, int D) {
   const size_t tiles = ((size_t)max_seq_len - 1) / kTile + 1;
   const size_t ctas = std::min<size_t>(kMaxCtas, tiles * B * Hkv * row_chunks(T, Hq, Hkv));
-  const size_t rows = T * (Hq / Hkv) <= 8 ? 8 : 16;
-  return kCounterBytes + ctas * (warps_of(D) + 2) * rows * (D + 10) * 4;
+  return workspace_of(ctas, T * (Hq / Hkv) <= 8 ? 8 : 16, D);
 }
 
 int check_cache(const focal_kv8_cache* c);
@@ -991,6 +1035,27 @@ int launch_decode(const CUtensorMap& mk, const CUtensorMap& mv, const DecodePara
 using namespace focal;
 
 extern "C" {
+
+int focal_kv8_decode_plan(int segs, int max_seq_len, int D, int code, int sm_count, int total, int top, int out[4]) {
+  using namespace kv8;
+  clear_error();
+  if (segs < 1 || sm_count < 1 || max_seq_len < 1 || top < 0 || total < 0 || !out)
+    return set_error(FOCAL_ERR_INVALID_VALUE, "segs, sm_count and max_seq_len must be positive");
+  if (D != 64 && D != 128) return set_error(FOCAL_ERR_UNSUPPORTED, "unsupported head_dim (must be 64 or 128)");
+  const Plan plan = plan_for(segs, (max_seq_len - 1) / kTile + 1, sm_count, D);
+  int ways = plan.ways, per = plan.per;
+  if (plan.decide) {
+    if (D == 128)
+      code == FOCAL_INT8 ? share_out<128, true>(plan, total, top, ways, per) : share_out<128, false>(plan, total, top, ways, per);
+    else
+      code == FOCAL_INT8 ? share_out<64, true>(plan, total, top, ways, per) : share_out<64, false>(plan, total, top, ways, per);
+  }
+  out[0] = plan.ctas;
+  out[1] = ways;
+  out[2] = per;
+  out[3] = (int)workspace_of(plan.ctas, 8, D);
+  return FOCAL_OK;
+}
 
 size_t focal_kv8_decode_counter_bytes(void) { return kv8::kCounterBytes; }
 
@@ -1032,23 +1097,8 @@ int focal_kv8_decode(const void* q, void* o, const focal_kv8_cache* cache, const
   const int per_seg = (max_seq_len - 1) / kTile + 1;
   const long long tiles = (long long)B * Hkv * p.chunks * per_seg;
   if (tiles > INT32_MAX / 2) return set_error(FOCAL_ERR_UNSUPPORTED, "B * Hkv * max_seq_len too large");
-  const int sms = std::min(dev.sm_count, kMaxCtas);
-  p.segs = B * Hkv * p.chunks;
-  p.stack = (p.segs - 1) / sms + 1;
-  p.ways = sms / p.segs;
-  if (p.ways > 0) {
-    // One CTA where its warps have hardly more than a tile each, or else parts of 4 tiles or more; and not so many
-    // that joining them (110 cycles each) costs more than it saves (560 a tile).
-    const int most = (int)(2.25 * std::sqrt((double)per_seg)) + 1;
-    p.ways = per_seg <= warps_of(D) * 3 / 2 ? 1 : std::min({p.ways, (per_seg + 3) / 4, most});
-    p.per = (per_seg + p.ways - 1) / p.ways;
-    p.ways = (per_seg + p.per - 1) / p.per;
-    p.by_ways.set(p.ways);
-  }
-  // parts this small cannot be uneven enough to matter
-  p.decide = p.ways == 0 || p.per > warps_of(D) * 3 / 2;
-  const int ctas = p.decide ? (int)std::min<long long>(std::max<long long>((tiles + 3) / 4, (long long)p.segs * p.ways), sms)
-                            : p.segs * p.ways;
+  p.plan = plan_for(B * Hkv * p.chunks, per_seg, dev.sm_count, D);
+  const int ctas = p.plan.ctas;
   p.q = q;
   p.o = o;
   p.k_scales = cache->k_scales;
@@ -1074,7 +1124,6 @@ int focal_kv8_decode(const void* q, void* o, const focal_kv8_cache* cache, const
   p.by_chunks.set(p.chunks);
   p.by_grp.set(p.grp);
   p.by_page.set(cache->page_size);
-  p.by_grid.set(ctas);
 
   // pages [num_pages, Hkv, page_size, D] of bytes; boxes of min(page_size, 64) rows
   CUtensorMap mk, mv;

@@ -351,6 +351,15 @@ int focal_kv8_decode(const void* q, void* o, const focal_kv8_cache* cache, const
                      const int32_t* seq_lens, int B, int T, int Hq, int max_pages_per_seq, int max_seq_len,
                      float scale, int dtype, void* workspace, size_t ws_bytes, cudaStream_t stream);
 
+/* How focal_kv8_decode shares out `segs` segments (a sequence, a KV head, up to
+ * 16 of its T * Hq / Hkv query rows) on sm_count SMs, where the longest has `top` tiles
+ * of 64 positions and all have `total` (diagnostics; no CUDA call).
+ *   out[0]  CTAs that are launched
+ *   out[1]  CTAs of a segment, 0: CTA c takes tiles c * out[2] .. of all, in one order
+ *   out[2]  tiles of a CTA
+ *   out[3]  bytes of workspace that it uses, for segments of up to 8 query rows */
+int focal_kv8_decode_plan(int segs, int max_seq_len, int D, int code, int sm_count, int total, int top, int out[4]);
+
 /* ------------------------------------------------------------ diagnostics ---
  * Device-side status word of the current device: 0 while every kernel's
  * bounded waits have completed; otherwise 1 (a pipeline wait gave up), 2 (a

@@ -967,6 +967,9 @@ int check_decode(int B, int T, int Hq, int Hkv, int max_seq_len, int D) {
   if (Hq % Hkv != 0) return set_error(FOCAL_ERR_UNSUPPORTED, "Hq must be a multiple of Hkv");
   if (Hq / Hkv > kMaxGroup) return set_error(FOCAL_ERR_UNSUPPORTED, "Hq / Hkv must be <= 16");
   if ((long long)B * Hkv > 65535) return set_error(FOCAL_ERR_UNSUPPORTED, "B * Hkv too large");
+  // tiles are counted in 32 bits
+  if ((long long)B * Hkv * row_chunks(T, Hq, Hkv) * ((max_seq_len - 1) / kTile + 1) > INT32_MAX / 2)
+    return set_error(FOCAL_ERR_UNSUPPORTED, "B * Hkv * max_seq_len too large");
   return FOCAL_OK;
 }
 
@@ -1095,8 +1098,6 @@ int focal_kv8_decode(const void* q, void* o, const focal_kv8_cache* cache, const
   DecodeParams p{};
   p.chunks = row_chunks(T, Hq, Hkv);
   const int per_seg = (max_seq_len - 1) / kTile + 1;
-  const long long tiles = (long long)B * Hkv * p.chunks * per_seg;
-  if (tiles > INT32_MAX / 2) return set_error(FOCAL_ERR_UNSUPPORTED, "B * Hkv * max_seq_len too large");
   p.plan = plan_for(B * Hkv * p.chunks, per_seg, dev.sm_count, D);
   const int ctas = p.plan.ctas;
   p.q = q;

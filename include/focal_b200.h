@@ -337,7 +337,8 @@ int focal_kv8_append(const focal_kv8_append_args* args, const focal_kv8_cache* c
  * lengths, so a sequence's result may differ in its last bits between batches;
  * equal calls give equal bits.
  * Contract: Hq % num_kv_heads == 0, Hq / num_kv_heads <= 16, 1 <= T <= 16,
- * max_seq_len <= 2^30.
+ * max_seq_len <= 2^30, B * Hkv <= 65535, and B * Hkv * ceil(T * Hq / Hkv / 16) *
+ * ceil(max_seq_len / 64) < 2^30; focal_kv8_decode_workspace_size() is 0 where it does not hold.
  *
  * Workspace: focal_kv8_decode_workspace_size() bytes, 256-byte aligned; its
  * first focal_kv8_decode_counter_bytes() bytes must be zero before the first

@@ -528,7 +528,7 @@ c10::optional<torch::Tensor> kv8_append(torch::Tensor k, torch::Tensor v, torch:
   return turned;
 }
 
-// The checks of kv8_attention; returns its workspace's size.
+// The checks of an attention call; returns its workspace's size.
 size_t check_attention(const torch::Tensor& q, int64_t B, int64_t T, const focal_kv8_cache& cache,
                        const torch::Tensor& block_table, const torch::Tensor& seq_lens, int64_t max_seq_len,
                        c10::optional<double> scale) {
@@ -545,20 +545,35 @@ size_t check_attention(const torch::Tensor& q, int64_t B, int64_t T, const focal
   return bytes;
 }
 
-// q, o [B * T, Hq, D] in any shape that ends so
-torch::Tensor kv8_attention(const torch::Tensor& q, int64_t B, int64_t T, int dtype, const focal_kv8_cache& cache,
-                            const torch::Tensor& block_table, const torch::Tensor& seq_lens, int64_t max_seq_len,
-                            c10::optional<double> scale) {
-  const size_t bytes = check_attention(q, B, T, cache, block_table, seq_lens, max_seq_len, scale);
-  const double sc = scale.has_value() ? *scale : 1.0 / std::sqrt((double)cache.head_dim);
+// What an attention call over q [B * T, Hq, D] (in any shape that ends so) needs: its checks are made, an
+// earlier call's device-side failure is reported and memory is allocated here, so that a
+// composite has all of it behind it before it writes to the cache.
+struct Kv8Attention {
+  torch::Tensor o, ws;
+  size_t bytes;
+  float scale;
+};
+
+Kv8Attention prepare_attention(const torch::Tensor& q, int64_t B, int64_t T, const focal_kv8_cache& cache,
+                               const torch::Tensor& block_table, const torch::Tensor& seq_lens, int64_t max_seq_len,
+                               c10::optional<double> scale) {
+  Kv8Attention a;
+  a.bytes = check_attention(q, B, T, cache, block_table, seq_lens, max_seq_len, scale);
+  a.scale = (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)cache.head_dim));
   const c10::cuda::CUDAGuard guard(q.device());
-  auto o = empty_like_rows(q);
-  const cudaStream_t stream = current_stream();
-  const auto ws = capturable_workspace(kWsKv8, q.device(), stream, bytes, focal_kv8_decode_counter_bytes());
-  raise_on(focal_kv8_decode(q.data_ptr(), o.data_ptr(), &cache, block_table.data_ptr<int32_t>(),
+  a.o = empty_like_rows(q);
+  a.ws = capturable_workspace(kWsKv8, q.device(), current_stream(), a.bytes, focal_kv8_decode_counter_bytes());
+  return a;
+}
+
+torch::Tensor run_attention(const Kv8Attention& a, const torch::Tensor& q, int64_t B, int64_t T, int dtype,
+                            const focal_kv8_cache& cache, const torch::Tensor& block_table,
+                            const torch::Tensor& seq_lens, int64_t max_seq_len) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  raise_on(focal_kv8_decode(q.data_ptr(), a.o.data_ptr(), &cache, block_table.data_ptr<int32_t>(),
                             seq_lens.data_ptr<int32_t>(), (int)B, (int)T, (int)q.size(-2), (int)block_table.size(1),
-                            (int)max_seq_len, (float)sc, dtype, ws.data_ptr(), bytes, stream));
-  return o;
+                            (int)max_seq_len, a.scale, dtype, a.ws.data_ptr(), a.bytes, current_stream()));
+  return a.o;
 }
 
 torch::Tensor gqa_decode_attention_kv8(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages,
@@ -569,12 +584,13 @@ torch::Tensor gqa_decode_attention_kv8(torch::Tensor q, torch::Tensor k_pages, t
   const int dtype = dtype_of(q, "q", false);
   TORCH_CHECK(q.dim() == 3 || q.dim() == 4, "q must have shape [B, Hq, D] or [B, T, Hq, D]");
   const focal_kv8_cache cache = kv8_cache_of(k_pages, v_pages, k_scales, v_scales, q, "q");
-  return kv8_attention(q, q.size(0), q.dim() == 4 ? q.size(1) : 1, dtype, cache, block_table, seq_lens, max_seq_len,
-                       scale);
+  const int64_t B = q.size(0), T = q.dim() == 4 ? q.size(1) : 1;
+  const Kv8Attention a = prepare_attention(q, B, T, cache, block_table, seq_lens, max_seq_len, scale);
+  return run_attention(a, q, B, T, dtype, cache, block_table, seq_lens, max_seq_len);
 }
 
-// A decode step's append and attention.  What the attention would refuse is
-// refused before the append writes to the cache.
+// A decode step's append and attention.  What the attention would refuse, an earlier call's failure
+// and a lack of memory are reported before the append writes to the cache.
 torch::Tensor decode_attention_kv8(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor k_pages,
                                    torch::Tensor v_pages, torch::Tensor k_scales, torch::Tensor v_scales,
                                    torch::Tensor block_table, torch::Tensor seq_lens, int64_t max_seq_len,
@@ -587,10 +603,10 @@ torch::Tensor decode_attention_kv8(torch::Tensor q, torch::Tensor k, torch::Tens
   const int64_t B = seq_lens.dim() == 1 ? seq_lens.size(0) : 0;
   TORCH_CHECK(B > 0 && k.size(0) % B == 0, "every sequence must have the same number of new tokens");
   const int64_t T = k.size(0) / B;
-  check_attention(q, B, T, cache, block_table, seq_lens, max_seq_len, scale);
+  const Kv8Attention a = prepare_attention(q, B, T, cache, block_table, seq_lens, max_seq_len, scale);
   const auto turned = kv8_append(k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, c10::nullopt, T, q,
                                  inv_freq, interleaved, mscale);
-  return kv8_attention(*turned, B, T, dtype, cache, block_table, seq_lens, max_seq_len, scale);
+  return run_attention(a, *turned, B, T, dtype, cache, block_table, seq_lens, max_seq_len);
 }
 
 }  // namespace

@@ -109,6 +109,14 @@ __device__ __forceinline__ uint32_t quantise4(const float* x, float scale, float
   return f32x2_to_e4m3x2(q[0], q[1]) | static_cast<uint32_t>(f32x2_to_e4m3x2(q[2], q[3])) << 16;
 }
 
+// The code of a value in a block of scale 0, whose finite values are zeros: infinities
+// saturate and NaN stays NaN there too.
+template <bool INT8>
+__device__ __forceinline__ uint32_t unscaled_code(float x) {
+  if (fabsf(x) == INFINITY) return INT8 ? (x > 0.f ? 0x7Fu : 0x81u) : (x > 0.f ? 0x7Eu : 0xFEu);
+  return !INT8 && x != x ? 0x7Fu : 0u;
+}
+
 template <bool INT8>
 __device__ __forceinline__ void dequantise4(uint32_t c, float (&x)[4]) {
   if (INT8) {
@@ -294,7 +302,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps, kBlocksPerSm) append_kernel
     }
     // Twice over the rows, for amax and for the codes: turning them again costs less than
     // the registers that would hold them.  Infinities saturate and NaN is stored as NaN
-    // (e4m3) or 0 (int8); neither sets the scale.
+    // (e4m3) or 0 (int8); neither sets the scale, which is 0 beside zeros alone.
     auto amax_of = [&](auto finite) {  // of all values (but NaN), or of the finite ones
       float amax = 0.f;
 #pragma unroll 1
@@ -333,10 +341,15 @@ __global__ void __launch_bounds__(32 * kAppendWarps, kBlocksPerSm) append_kernel
       const int r = i * kRows + rr;
       values(i, val);
       if (r >= r0 && r < r1) {
-        uint32_t w[4] = {0u, 0u, 0u, 0u};
+        uint32_t w[4];
         if (scale > 0.f) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) w[e] = quantise4<INT8>(val + 4 * e, scale, inv, exact);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[e] = unscaled_code<INT8>(val[4 * e]) | unscaled_code<INT8>(val[4 * e + 1]) << 8 |
+                   unscaled_code<INT8>(val[4 * e + 2]) << 16 | unscaled_code<INT8>(val[4 * e + 3]) << 24;
         }
         *reinterpret_cast<uint2*>(out + r * D + d0) = make_uint2(w[0], w[1]);
         *reinterpret_cast<uint2*>(out + r * D + d1) = make_uint2(w[2], w[3]);

@@ -302,8 +302,9 @@ typedef struct focal_kv8_cache {
  *   block's first row is among the new; code = nearest-even(x / scale).
  * If the scale grows, the codes of the block's older rows are moved to it.
  * Rows behind a sequence's last token are left as they were.  Infinities
- * saturate; NaN becomes e4m3's NaN or int8's 0.  All the rows appended to a page
- * must belong to one sequence of the call.
+ * saturate, to the largest code; NaN becomes e4m3's NaN or int8's 0; neither counts
+ * for amax (beside zeros alone the scale is 0, and a saturated infinity stands for 0).
+ * All the rows appended to a page must belong to one sequence of the call.
  *
  * Rows of q_out that belong to no sequence are not written.
  *

@@ -43,9 +43,7 @@ def needed_scale(amax: float, code: torch.dtype) -> float:
 
 def quantise(x, scale: float, code: torch.dtype):
     """The codes of x / scale (as float64 numbers), nearest even, saturating."""
-    if scale == 0.0:
-        return torch.zeros_like(x)
-    r = x / scale
+    r = x / (scale or 1.0)  # scale 0: zeros, infinities and NaN
     if code == torch.int8:
         return r.round().clamp(-127, 127)
     # e4m3: three mantissa bits, smallest exponent -6

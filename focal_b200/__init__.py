@@ -231,7 +231,8 @@ def rope_inv_freq(rot: int, base: float = 10000.0, scaling: str | None = None, f
       "yarn"    pairs that turn less than `low` times over the original length
                 are divided by factor, those that turn more than `high` times
                 are kept, with a linear ramp over the pairs between (rounded
-                outwards to whole pairs); mscale is 0.1 ln(factor) + 1
+                outwards to whole pairs, and up to rot - 1: it may end behind the
+                last pair, which is then divided in part); mscale is 0.1 ln(factor) + 1
       "bands"   as "yarn" with the ramp in the number of turns itself, from `low`
                 to `high`; mscale is 1
     """
@@ -255,7 +256,7 @@ def rope_inv_freq(rot: int, base: float = 10000.0, scaling: str | None = None, f
             def pair(turns):  # the fractional pair that turns so often over the original length
                 return rot * math.log(original_max_position / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-            first, last = max(math.floor(pair(high)), 0), min(math.ceil(pair(low)), rot // 2 - 1)
+            first, last = max(math.floor(pair(high)), 0), min(math.ceil(pair(low)), rot - 1)
             keep = [1.0 - min(1.0, max(0.0, (i - first) / max(last - first, 0.001))) for i in range(rot // 2)]
             mscale = 0.1 * math.log(factor) + 1.0
         else:

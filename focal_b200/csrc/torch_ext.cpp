@@ -88,29 +88,79 @@ torch::Tensor workspace_for(WsKind kind, const torch::Device& dev, cudaStream_t 
 }
 
 // A workspace for a call that may be captured.  Outside a capture it is
-// workspace_for's.  Inside one it belongs to that capture and stream: allocated
-// from the graph's own pool, its counters zeroed by a node of the graph, so
-// graphs that replay at the same time share nothing and a graph's replay does
-// not depend on what the workspace held.  The tensor is kept until another
-// capture on the stream begins; the memory itself lives as long as its graph.
-std::map<std::pair<int, cudaStream_t>, std::pair<unsigned long long, torch::Tensor>> g_capture_ws;
+// workspace_for's.  Inside one it belongs to that capture and stream: its counters are
+// zeroed by a node of the graph, so graphs that replay at the same time share
+// nothing and a graph's replay does not depend on what the workspace held.  The
+// graph holds a reference to the tensor (a user object), so its memory lives as
+// long as the graph and what was instantiated from it, whoever began the capture and
+// whatever pool it came from.  The reference is given back on a thread that
+// may not call CUDA; the tensor waits on a list for the next call to free it.
+struct CaptureWs {
+  unsigned long long id = 0;        // the capture
+  torch::Tensor* tensor = nullptr;  // the graph's: there while the capture is
+};
+std::map<std::pair<int, cudaStream_t>, CaptureWs> g_capture_ws;
+
+struct DroppedList {
+  std::mutex mutex;
+  std::vector<torch::Tensor*> tensors;
+};
+DroppedList& dropped() {
+  static DroppedList* const list = new DroppedList;  // never destroyed: graphs may outlive static objects
+  return *list;
+}
+
+void drop_tensor(void* t) {
+  std::lock_guard<std::mutex> lock(dropped().mutex);
+  dropped().tensors.push_back(static_cast<torch::Tensor*>(t));
+}
+
+void free_dropped() {
+  std::vector<torch::Tensor*> list;
+  {
+    std::lock_guard<std::mutex> lock(dropped().mutex);
+    list.swap(dropped().tensors);
+  }
+  for (torch::Tensor* t : list) delete t;
+}
+
+// A tensor that `graph`, which is being captured, keeps.
+torch::Tensor* kept_by(cudaGraph_t graph, torch::Tensor tensor) {
+  auto* t = new torch::Tensor(std::move(tensor));
+  cudaUserObject_t object = nullptr;
+  cudaError_t e = cudaUserObjectCreate(&object, t, drop_tensor, 1, cudaUserObjectNoDestructorSync);
+  if (e != cudaSuccess) {
+    delete t;
+    TORCH_CHECK(false, "cudaUserObjectCreate: ", cudaGetErrorString(e));
+  }
+  e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+  if (e != cudaSuccess) {
+    cudaUserObjectRelease(object, 1);
+    TORCH_CHECK(false, "cudaGraphRetainUserObject: ", cudaGetErrorString(e));
+  }
+  return t;
+}
 
 torch::Tensor capturable_workspace(WsKind kind, const torch::Device& dev, cudaStream_t stream, size_t bytes,
                                    size_t counter_bytes) {
+  free_dropped();
   cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
   unsigned long long id = 0;
-  cudaError_t e = cudaStreamGetCaptureInfo(stream, &st, &id);
+  cudaGraph_t graph = nullptr;
+  cudaError_t e = cudaStreamGetCaptureInfo(stream, &st, &id, &graph);
   TORCH_CHECK(e == cudaSuccess, "cudaStreamGetCaptureInfo: ", cudaGetErrorString(e));
   if (st == cudaStreamCaptureStatusNone) return workspace_for(kind, dev, stream, bytes);
+  TORCH_CHECK(st == cudaStreamCaptureStatusActive, "the stream's capture has been invalidated");
   std::lock_guard<std::mutex> lock(g_ws_mutex);
-  auto& slot = g_capture_ws[std::make_pair((int)dev.index(), stream)];
-  if (!slot.second.defined() || slot.first != id || (size_t)slot.second.numel() < bytes) {
-    slot.second = torch::empty({(int64_t)bytes}, torch::TensorOptions().dtype(torch::kUInt8).device(dev));
-    slot.first = id;
-    e = cudaMemsetAsync(slot.second.data_ptr(), 0, std::min(bytes, counter_bytes), stream);
+  CaptureWs& slot = g_capture_ws[std::make_pair((int)dev.index(), stream)];
+  if (slot.tensor == nullptr || slot.id != id || (size_t)slot.tensor->numel() < bytes) {
+    auto t = torch::empty({(int64_t)bytes}, torch::TensorOptions().dtype(torch::kUInt8).device(dev));
+    e = cudaMemsetAsync(t.data_ptr(), 0, std::min(bytes, counter_bytes), stream);
     TORCH_CHECK(e == cudaSuccess, "cudaMemsetAsync (workspace): ", cudaGetErrorString(e));
+    slot.tensor = kept_by(graph, std::move(t));
+    slot.id = id;
   }
-  return slot.second;
+  return *slot.tensor;
 }
 
 // For calls without a workspace: report an earlier call's device-side failure.
@@ -468,11 +518,14 @@ void check_tables(const torch::Tensor& block_table, const torch::Tensor& seq_len
   TORCH_CHECK(B <= INT32_MAX && block_table.size(1) <= INT32_MAX, "unsupported size");
 }
 
-c10::optional<torch::Tensor> kv8_append(torch::Tensor k, torch::Tensor v, torch::Tensor k_pages, torch::Tensor v_pages,
-                                        torch::Tensor k_scales, torch::Tensor v_scales, torch::Tensor block_table,
-                                        torch::Tensor seq_lens, c10::optional<torch::Tensor> cu_new, int64_t max_new,
-                                        c10::optional<torch::Tensor> q, c10::optional<torch::Tensor> inv_freq,
-                                        bool interleaved, double mscale) {
+// The turned q goes to q_out where the caller has a place for it, else to a tensor that is returned.
+c10::optional<torch::Tensor> append_rows(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& k_pages,
+                                         const torch::Tensor& v_pages, const torch::Tensor& k_scales,
+                                         const torch::Tensor& v_scales, const torch::Tensor& block_table,
+                                         const torch::Tensor& seq_lens, const c10::optional<torch::Tensor>& cu_new,
+                                         int64_t max_new, const c10::optional<torch::Tensor>& q, void* q_out,
+                                         const c10::optional<torch::Tensor>& inv_freq, bool interleaved,
+                                         double mscale) {
   check_rows(k, "k", k);
   check_rows(v, "v", k);
   focal_kv8_append_args a{};
@@ -502,9 +555,9 @@ c10::optional<torch::Tensor> kv8_append(torch::Tensor k, torch::Tensor v, torch:
     check_rows(*q, "q", k);
     TORCH_CHECK(inv_freq.has_value(), "q needs inv_freq: it is only turned");
     TORCH_CHECK(q->size(0) == T && q->size(2) == k.size(2), "q must have shape [T, Hq, D]");
-    turned = empty_like_rows(*q);
+    if (!q_out) turned = empty_like_rows(*q);
     a.q = q->data_ptr();
-    a.q_out = turned->data_ptr();
+    a.q_out = q_out ? q_out : turned->data_ptr();
     a.Hq = (int)q->size(1);
     a.q_token_stride = stride_of(*q, 0);
     a.q_head_stride = stride_of(*q, 1);
@@ -528,6 +581,15 @@ c10::optional<torch::Tensor> kv8_append(torch::Tensor k, torch::Tensor v, torch:
   return turned;
 }
 
+c10::optional<torch::Tensor> kv8_append(torch::Tensor k, torch::Tensor v, torch::Tensor k_pages, torch::Tensor v_pages,
+                                        torch::Tensor k_scales, torch::Tensor v_scales, torch::Tensor block_table,
+                                        torch::Tensor seq_lens, c10::optional<torch::Tensor> cu_new, int64_t max_new,
+                                        c10::optional<torch::Tensor> q, c10::optional<torch::Tensor> inv_freq,
+                                        bool interleaved, double mscale) {
+  return append_rows(k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, cu_new, max_new, q, nullptr,
+                     inv_freq, interleaved, mscale);
+}
+
 // The checks of an attention call; returns its workspace's size.
 size_t check_attention(const torch::Tensor& q, int64_t B, int64_t T, const focal_kv8_cache& cache,
                        const torch::Tensor& block_table, const torch::Tensor& seq_lens, int64_t max_seq_len,
@@ -547,32 +609,38 @@ size_t check_attention(const torch::Tensor& q, int64_t B, int64_t T, const focal
 
 // What an attention call over q [B * T, Hq, D] (in any shape that ends so) needs: its checks are made, an
 // earlier call's device-side failure is reported and memory is allocated here, so that a
-// composite has all of it behind it before it writes to the cache.
+// composite has all of it behind it before it writes to the cache.  With `rows`, the workspace has
+// room for q's rows too, at `turned`: nothing but outputs lies in memory that a captured
+// graph does not keep.
 struct Kv8Attention {
   torch::Tensor o, ws;
   size_t bytes;
   float scale;
+  void* turned;
 };
 
 Kv8Attention prepare_attention(const torch::Tensor& q, int64_t B, int64_t T, const focal_kv8_cache& cache,
                                const torch::Tensor& block_table, const torch::Tensor& seq_lens, int64_t max_seq_len,
-                               c10::optional<double> scale) {
+                               c10::optional<double> scale, bool rows) {
   Kv8Attention a;
   a.bytes = check_attention(q, B, T, cache, block_table, seq_lens, max_seq_len, scale);
   a.scale = (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)cache.head_dim));
   const c10::cuda::CUDAGuard guard(q.device());
   a.o = empty_like_rows(q);
-  a.ws = capturable_workspace(kWsKv8, q.device(), current_stream(), a.bytes, focal_kv8_decode_counter_bytes());
+  const size_t at = (a.bytes + 255) / 256 * 256;
+  a.ws = capturable_workspace(kWsKv8, q.device(), current_stream(), rows ? at + (size_t)a.o.nbytes() : a.bytes,
+                              focal_kv8_decode_counter_bytes());
+  a.turned = rows ? static_cast<uint8_t*>(a.ws.data_ptr()) + at : nullptr;
   return a;
 }
 
-torch::Tensor run_attention(const Kv8Attention& a, const torch::Tensor& q, int64_t B, int64_t T, int dtype,
+torch::Tensor run_attention(const Kv8Attention& a, const void* q, int64_t B, int64_t T, int dtype,
                             const focal_kv8_cache& cache, const torch::Tensor& block_table,
                             const torch::Tensor& seq_lens, int64_t max_seq_len) {
-  const c10::cuda::CUDAGuard guard(q.device());
-  raise_on(focal_kv8_decode(q.data_ptr(), a.o.data_ptr(), &cache, block_table.data_ptr<int32_t>(),
-                            seq_lens.data_ptr<int32_t>(), (int)B, (int)T, (int)q.size(-2), (int)block_table.size(1),
-                            (int)max_seq_len, a.scale, dtype, a.ws.data_ptr(), a.bytes, current_stream()));
+  const c10::cuda::CUDAGuard guard(a.o.device());
+  raise_on(focal_kv8_decode(q, a.o.data_ptr(), &cache, block_table.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(),
+                            (int)B, (int)T, (int)a.o.size(-2), (int)block_table.size(1), (int)max_seq_len, a.scale, dtype,
+                            a.ws.data_ptr(), a.bytes, current_stream()));
   return a.o;
 }
 
@@ -585,8 +653,8 @@ torch::Tensor gqa_decode_attention_kv8(torch::Tensor q, torch::Tensor k_pages, t
   TORCH_CHECK(q.dim() == 3 || q.dim() == 4, "q must have shape [B, Hq, D] or [B, T, Hq, D]");
   const focal_kv8_cache cache = kv8_cache_of(k_pages, v_pages, k_scales, v_scales, q, "q");
   const int64_t B = q.size(0), T = q.dim() == 4 ? q.size(1) : 1;
-  const Kv8Attention a = prepare_attention(q, B, T, cache, block_table, seq_lens, max_seq_len, scale);
-  return run_attention(a, q, B, T, dtype, cache, block_table, seq_lens, max_seq_len);
+  const Kv8Attention a = prepare_attention(q, B, T, cache, block_table, seq_lens, max_seq_len, scale, false);
+  return run_attention(a, q.data_ptr(), B, T, dtype, cache, block_table, seq_lens, max_seq_len);
 }
 
 // A decode step's append and attention.  What the attention would refuse, an earlier call's failure
@@ -603,10 +671,10 @@ torch::Tensor decode_attention_kv8(torch::Tensor q, torch::Tensor k, torch::Tens
   const int64_t B = seq_lens.dim() == 1 ? seq_lens.size(0) : 0;
   TORCH_CHECK(B > 0 && k.size(0) % B == 0, "every sequence must have the same number of new tokens");
   const int64_t T = k.size(0) / B;
-  const Kv8Attention a = prepare_attention(q, B, T, cache, block_table, seq_lens, max_seq_len, scale);
-  const auto turned = kv8_append(k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, c10::nullopt, T, q,
-                                 inv_freq, interleaved, mscale);
-  return run_attention(a, *turned, B, T, dtype, cache, block_table, seq_lens, max_seq_len);
+  const Kv8Attention a = prepare_attention(q, B, T, cache, block_table, seq_lens, max_seq_len, scale, true);
+  append_rows(k, v, k_pages, v_pages, k_scales, v_scales, block_table, seq_lens, c10::nullopt, T, q, a.turned, inv_freq,
+              interleaved, mscale);
+  return run_attention(a, a.turned, B, T, dtype, cache, block_table, seq_lens, max_seq_len);
 }
 
 }  // namespace

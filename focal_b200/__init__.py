@@ -278,7 +278,8 @@ def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, inter
     QKV rows will do); positions int32 or int64 [T]; inv_freq fp64.  Angles (below 2^50), cos
     and sin are 64-bit, the turn fp32, with one rounding.  Writes a new
     contiguous tensor, or `out` (x itself works in place, any other overlap
-    does not).  For inference: it has no gradient.
+    does not).  For inference: it has no gradient, and refuses an x that requires
+    one (detach it, or call under torch.no_grad()); so do the calls below.
     """
     return _ext().rope(x, positions, inv_freq, interleaved, mscale, out)
 

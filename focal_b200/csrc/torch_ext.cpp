@@ -418,6 +418,12 @@ int dtype_of(const torch::Tensor& t, const char* name, bool fp32) {
   return FOCAL_FP32;
 }
 
+// These calls have no gradient; a tensor that expects one is refused rather than cut off.
+void check_no_grad(const torch::Tensor& t, const char* name) {
+  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name,
+              " requires a gradient, which this call does not have: detach it, or call under torch.no_grad()");
+}
+
 // [tokens, heads, D] rows: the last dimension contiguous, the others strided.
 void check_rows(const torch::Tensor& t, const char* name, const torch::Tensor& like) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
@@ -425,6 +431,7 @@ void check_rows(const torch::Tensor& t, const char* name, const torch::Tensor& l
   TORCH_CHECK(t.size(2) <= 1 || t.stride(2) == 1, name, " must have a contiguous last dimension");
   TORCH_CHECK(t.device() == like.device(), "all tensors must be on ", name, "'s device");
   TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " has wrong dtype");
+  check_no_grad(t, name);
   TORCH_CHECK(t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX && t.size(2) <= INT32_MAX, "unsupported size");
 }
 
@@ -649,6 +656,7 @@ torch::Tensor gqa_decode_attention_kv8(torch::Tensor q, torch::Tensor k_pages, t
                                        torch::Tensor seq_lens, int64_t max_seq_len, c10::optional<double> scale) {
   TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
   TORCH_CHECK(q.is_contiguous(), "q must be contiguous");
+  check_no_grad(q, "q");
   const int dtype = dtype_of(q, "q", false);
   TORCH_CHECK(q.dim() == 3 || q.dim() == 4, "q must have shape [B, Hq, D] or [B, T, Hq, D]");
   const focal_kv8_cache cache = kv8_cache_of(k_pages, v_pages, k_scales, v_scales, q, "q");

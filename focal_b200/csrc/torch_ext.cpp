@@ -79,7 +79,10 @@ torch::Tensor workspace_for(WsKind kind, const torch::Device& dev, cudaStream_t 
   auto key = std::make_tuple((int)kind, (int)dev.index(), stream);
   auto it = g_ws.find(key);
   if (it == g_ws.end() || (size_t)it->second.numel() < bytes) {
-    if (it != g_ws.end()) g_ws_retired.push_back(it->second);
+    if (it != g_ws.end()) {  // at least doubled, so that batches that grow step by step retire few of them
+      g_ws_retired.push_back(it->second);
+      bytes = std::max(bytes, 2 * (size_t)it->second.numel());
+    }
     auto t = torch::zeros({(int64_t)bytes}, torch::TensorOptions().dtype(torch::kUInt8).device(dev));
     g_ws[key] = t;
     return t;

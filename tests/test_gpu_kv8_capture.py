@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import focal_b200 as F
+from focal_b200 import _lib
 from test_gpu_kv8 import clones, gen, ints, random_cache, same, status, table_for
 
 pytestmark = pytest.mark.gpu
@@ -128,4 +129,26 @@ def test_what_a_graph_kept_is_freed_behind_it(cuda):
                 break
             time.sleep(0.05)
         assert torch.cuda.memory_allocated() == base
+    assert status() == 0
+
+
+def test_steps_of_growing_batches_hold_little_memory(cuda):
+    """Eager steps of one sequence more from call to call: the workspaces that the stream outgrows (kept for
+    graphs) double at least, so all of them take less than four times the largest that is needed."""
+    f, _ = F.rope_inv_freq(128, device=cuda)
+    most = 200
+    cache = F.kv8_cache(most, 2, 16, 128, device=cuda)
+    table = torch.arange(most, dtype=torch.int32, device=cuda).view(most, 1)
+    lens = torch.full((most,), 7, dtype=torch.int32, device=cuda)
+    x = torch.randn(most, 36, 128, device=cuda, generator=gen(cuda, 1)).to(BF16)
+    run = lambda b: F.decode_attention_kv8(x[:b, :32], x[:b, 32:34], x[:b, 34:], cache, table[:b], lens[:b], 16, f)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        base = torch.cuda.memory_allocated()
+        for b in range(1, most + 1):
+            run(b)
+        need = _lib.lib().focal_kv8_decode_workspace_size(most, 1, 32, 2, 16, 128)
+        assert torch.cuda.memory_allocated() - base < 4 * need
+        torch.cuda.synchronize()
     assert status() == 0

@@ -619,11 +619,12 @@ size_t check_attention(const torch::Tensor& q, int64_t B, int64_t T, const focal
 
 // What an attention call over q [B * T, Hq, D] (in any shape that ends so) needs: its checks are made, an
 // earlier call's device-side failure is reported and memory is allocated here, so that a
-// composite has all of it behind it before it writes to the cache.  With `rows`, the workspace has
-// room for q's rows too, at `turned`: nothing but outputs lies in memory that a captured
-// graph does not keep.
+// composite has all of it behind it before it writes to the cache.  With `rows` there is
+// room for q's rows too, at `turned`: under a capture in the workspace, so that nothing but outputs
+// lies in memory that the graph does not keep; else in a tensor of the call's own (the stream's workspace
+// would be outgrown, and retired, with every larger batch).
 struct Kv8Attention {
-  torch::Tensor o, ws;
+  torch::Tensor o, ws, rows;
   size_t bytes;
   float scale;
   void* turned;
@@ -637,10 +638,12 @@ Kv8Attention prepare_attention(const torch::Tensor& q, int64_t B, int64_t T, con
   a.scale = (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)cache.head_dim));
   const c10::cuda::CUDAGuard guard(q.device());
   a.o = empty_like_rows(q);
+  const bool inside = rows && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
   const size_t at = (a.bytes + 255) / 256 * 256;
-  a.ws = capturable_workspace(kWsKv8, q.device(), current_stream(), rows ? at + (size_t)a.o.nbytes() : a.bytes,
+  if (rows && !inside) a.rows = empty_like_rows(q);
+  a.ws = capturable_workspace(kWsKv8, q.device(), current_stream(), inside ? at + (size_t)a.o.nbytes() : a.bytes,
                               focal_kv8_decode_counter_bytes());
-  a.turned = rows ? static_cast<uint8_t*>(a.ws.data_ptr()) + at : nullptr;
+  a.turned = !rows ? nullptr : inside ? static_cast<uint8_t*>(a.ws.data_ptr()) + at : a.rows.data_ptr();
   return a;
 }
 

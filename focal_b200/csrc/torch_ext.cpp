@@ -54,11 +54,18 @@ std::vector<torch::Tensor> g_ws_retired;
 // word is read (mapped host memory, no device sync); when it is set, every
 // cached workspace of the device is zeroed again on its own stream, the word is
 // cleared and the call raises, so the failure is reported once and later calls
-// are valid.  Called with g_ws_mutex held.
+// are valid.  In a capture, where the zeroing could become a node of the graph instead, the
+// call raises and leaves all of it to the next call outside.  Called with g_ws_mutex held.
 void check_device_status_locked(const torch::Device& dev) {
   int st = 0;
   raise_on(focal_device_status_peek(&st));
   if (st == 0) return;
+  const char* what =
+      st == 2 ? ": a tensor-parallel peer did not deliver" : st == 3 ? ": bad paged-KV index" : ": pipeline wait";
+  TORCH_CHECK(c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None,
+              "focal_b200: an earlier call on cuda:", (int)dev.index(),
+              " gave up a bounded device-side wait (status ", st, what,
+              "); nothing is captured before a call outside the capture has cleared the status.");
   for (auto& kv : g_ws)
     if (std::get<1>(kv.first) == (int)dev.index()) {
       const cudaError_t e =
@@ -67,8 +74,7 @@ void check_device_status_locked(const torch::Device& dev) {
     }
   raise_on(focal_reset_device_status());
   TORCH_CHECK(false, "focal_b200: an earlier call on cuda:", (int)dev.index(),
-              " gave up a bounded device-side wait (status ", st,
-              st == 2 ? ": a tensor-parallel peer did not deliver" : st == 3 ? ": bad paged-KV index" : ": pipeline wait",
+              " gave up a bounded device-side wait (status ", st, what,
               "); its output is invalid.  The cached workspaces were zeroed again and the status cleared; "
               "later calls are valid.");
 }

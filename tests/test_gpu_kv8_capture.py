@@ -152,3 +152,28 @@ def test_steps_of_growing_batches_hold_little_memory(cuda):
         assert torch.cuda.memory_allocated() - base < 4 * need
         torch.cuda.synchronize()
     assert status() == 0
+
+
+def test_a_failure_is_not_cleared_inside_a_capture(cuda):
+    """A call that is being captured reports an earlier failure and leaves it to a call outside to clear:
+    the stream's workspace cannot be zeroed in between."""
+    cache = random_cache(4, 2, 16, 128, E4M3, cuda, seed=1)
+    k = torch.ones(1, 2, 128, device=cuda, dtype=BF16)
+    q = torch.ones(1, 8, 128, device=cuda, dtype=BF16)
+    one, good, bad = ints([1], cuda), ints([[2]], cuda), ints([[4]], cuda)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = F.gqa_decode_attention_kv8(q, cache, good, one, 16)
+        F.kv8_append(k, k, cache, bad, one)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="bad paged-KV index.*outside the capture"):
+        with torch.cuda.graph(g, stream=side):
+            F.kv8_append(k, k, cache, good, one)
+    assert status() == 3
+    with torch.cuda.stream(side):
+        with pytest.raises(RuntimeError, match="bad paged-KV index.*later calls are valid"):
+            F.gqa_decode_attention_kv8(q, cache, good, one, 16)
+        assert torch.equal(F.gqa_decode_attention_kv8(q, cache, good, one, 16), want)
+    assert status() == 0

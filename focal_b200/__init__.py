@@ -345,7 +345,9 @@ def gqa_decode_attention_kv8(q: torch.Tensor, cache, block_table: torch.Tensor, 
     (query t sees positions < seq_lens[b] - T + 1 + t), bf16 or fp16; cache as
     kv8_append writes it; block_table int32 [B, max_pages]; seq_lens int32 [B] in
     0..max_seq_len (a host integer that sizes the launch).  A query that sees no
-    position gives zeros.  D is 64 or 128; scale defaults to 1/sqrt(D).
+    position gives zeros.  D is 64 or 128; scale defaults to 1/sqrt(D).  Scores, softmax
+    statistics and sums are fp32; a softmax weight enters the product with V with 11
+    bits for bf16 outputs, with 22 for fp16 ones.
     """
     return _ext().gqa_decode_attention_kv8(q, *cache, block_table, seq_lens, max_seq_len, scale)
 

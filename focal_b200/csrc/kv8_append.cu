@@ -22,8 +22,10 @@
 // the next job's rows are on their way to shared memory; a lane has 16 dims of
 // every (32 / (D / 16))-th row.  K and V pass over their rows twice, for amax and for
 // the codes, from shared memory.  The cos and sin of the block's rows are computed
-// once per thread block into shared memory: of many rows, eight follow from one angle by
-// turning it on by inv_freq in 64 bits.
+// once per thread block into shared memory: of more than four rows, eight follow from one angle by
+// turning it on by inv_freq in 64 bits.  Seven such turns are off by less than 8 * 2^-45, and by
+// the rounding of the first angle; beside rope's own angle for each row, one cos or sin in some
+// thirty thousand rounds to another fp32 number (positions to 131072).
 //
 // Bound: HBM and the issue of some 800 instructions a job for prompts (8 x 1024
 // tokens of 32 + 16 heads 34.0 us, 0.83 of the measured copy rate; 5072 tokens in

@@ -72,8 +72,9 @@ __device__ __forceinline__ uint16_t f32x2_to_e4m3x2(float lo, float hi) {
 
 // cos and sin of a 64-bit angle, |a| < 2^50: less the nearest multiple of pi / 2,
 // which is subtracted in two parts (Cody and Waite), their Taylor series to
-// x^14 and x^13, off by less than 2^-45.  (CUDA's sincos is more exact and for any
-// angle, and took seven times as long; the result is rounded to fp32.)
+// x^14 and x^13, off by less than 2^-45: the rounding to fp32 that follows is then off by at
+// most 2^-25 + 2^-45 of values up to 1.  (CUDA's sincos is more exact and for any angle, and took
+// seven times as long.)
 __device__ __forceinline__ void cos_sin(double a, double& c, double& s) {
   constexpr double kShift = 6755399441055744.0;  // 1.5 2^52: the sum's low bits are the rounded integer
   const double t = fma(a, 0.63661977236758134308, kShift);

@@ -23,13 +23,17 @@
 //    one ring only.  (One producer warp with a ring for all streamed at 0.56 of the
 //    measured copy rate, this at 1.04: 8 sequences of 131072 tokens 591 and 317 us.  Seven
 //    warps with two whole tiles each, which left one scheduler half idle and HBM waiting for
-//    the first tiles' work: 16 ragged sequences 24.6 us instead of 21.9.)
+//    the first tiles' work: 16 ragged sequences 24.6 us, eight warps with half tiles 21.9, both with
+//    weights of one f16 number.)
 //  * The products are transposed: S^T = K Q^T and O^T = V^T P^T.  The 16-row side
 //    of mma.sync m16n8k16 holds positions and dims, its 8-column side the query rows
 //    (T * Hq / Hkv, 8 or 16 of them), which halves the products that 4 or 8
-//    query rows would need as the 16-row side.  (A tcgen05 tile's 64 or 128 rows
-//    would be as empty, and its operands would have to be converted through
-//    shared memory first.)
+//    query rows would need as the 16-row side.  (In this form a tcgen05 tile's 64 or 128
+//    rows would be full too, with the query rows as its N side; but its operands come from shared
+//    memory, so all codes would have to be written there once more as f16, for 8 or 16 query rows that
+//    mma.sync serves at 18 % of the tensor pipe.  Not measured.)
+//  * More than 16 query rows of a KV head are segments of their own, each of which streams and
+//    converts K and V again: 8 sequences of 4096 take 22 us with 16 rows, 30 with 32 and 170 with 256.
 //  * Codes become f16 exactly.  K's words are read 16 bytes a lane as they lie: the
 //    sum over dims may run in any order, so q is loaded in the same order.  V's
 //    come through ldmatrix.trans as pairs of dims, and the two bytes of a pair
@@ -43,10 +47,10 @@
 //    outputs it enters as two numbers, that and f16 of the rest: rounding the weights once
 //    is off by as much as rounding the output (together 1.4 times it, up to 2.6 times for a
 //    sequence of one; 16 ragged sequences 21.7 -> 22.5 us, 8 of up to 8191 with 4 tokens
-//    27.9 -> 30.7).  For bf16 outputs it is an eighth of that.
+//    27.9 -> 30.7).  For bf16 outputs it is an eighth of that: the outputs' error grows by about 1 %.
 // What is left: launch, lengths, page ids and the first tiles one after another
 // (about 4 us), and merge and join at the end (1 to 3 us); one sequence of 512
-// takes 5.8 us, 16 ragged ones of up to 4096 21.7 where their bytes take 11.4.
+// takes 5.8 us, as do 32 of 64; 16 ragged ones of up to 4096 (int8, fp16) 22.5 where their bytes take 11.4.
 #include <algorithm>
 #include <cmath>
 #include <cstring>

@@ -294,7 +294,9 @@ typedef struct focal_kv8_cache {
  * cu_new[b + 1] - 1 of k and v (without cu_new: max_new rows each, in order),
  * and become its last positions, seq_lens[b] - n .. seq_lens[b] - 1 (seq_lens
  * counts them already).  With rot > 0, k is turned by its positions first (see
- * focal_rope), and so is q into q_out, both from the same tokens.
+ * focal_rope), and so is q into q_out, both from the same tokens.  Of more than four new
+ * rows of a block some get their cos and sin by turning the row's before on, in 64 bits: the last
+ * fp32 bit of one in some thirty thousand differs from that of the same row appended alone.
  *
  * For the new rows of a block of 16 tokens and a head, amax = max |x|;
  *   e4m3: need = the smallest power of two >= amax / 448; int8: amax / 127
@@ -330,8 +332,10 @@ int focal_kv8_append(const focal_kv8_append_args* args, const focal_kv8_cache* c
 /* Attention of T query tokens per sequence, its last T positions, over the
  * cache: query token t of sequence b sees positions < seq_lens[b] - T + 1 + t.
  *   q, o [B, T, Hq, head_dim] of dtype (bf16 or fp16), contiguous
- * fp32 scores, softmax and accumulation; split over the positions with a
- * log-sum-exp combine in split order.  A query that sees no position gives 0.
+ * fp32 scores, softmax statistics and accumulation.  In the product with V a softmax weight
+ * (times its V scale) has 11 bits, one f16 number, for bf16 outputs, whose own rounding is
+ * eight times as large, and 22 bits, two f16 numbers, for fp16 outputs.  Split over the positions
+ * with a log-sum-exp combine in split order.  A query that sees no position gives 0.
  * seq_lens[b] is 0 .. max_seq_len <= max_pages_per_seq * page_size (block
  * table entries and rows past a sequence's end are not read as data).  Scales
  * must not be negative.  Which tiles are summed together depends on the whole batch's

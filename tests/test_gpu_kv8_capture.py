@@ -170,6 +170,7 @@ def test_a_failure_is_not_cleared_inside_a_capture(cuda):
     g = torch.cuda.CUDAGraph()
     with pytest.raises(RuntimeError, match="bad paged-KV index.*outside the capture"):
         with torch.cuda.graph(g, stream=side):
+            k.mul_(1.0)  # (a graph with a node)
             F.kv8_append(k, k, cache, good, one)
     assert status() == 3
     with torch.cuda.stream(side):

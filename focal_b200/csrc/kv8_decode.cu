@@ -1046,10 +1046,16 @@ extern "C" {
 int focal_kv8_decode_plan(int segs, int max_seq_len, int D, int code, int sm_count, int total, int top, int out[4]) {
   using namespace kv8;
   clear_error();
-  if (segs < 1 || sm_count < 1 || max_seq_len < 1 || top < 0 || total < 0 || !out)
+  if (segs < 1 || sm_count < 1 || max_seq_len < 1 || !out)
     return set_error(FOCAL_ERR_INVALID_VALUE, "segs, sm_count and max_seq_len must be positive");
   if (D != 64 && D != 128) return set_error(FOCAL_ERR_UNSUPPORTED, "unsupported head_dim (must be 64 or 128)");
-  const Plan plan = plan_for(segs, (max_seq_len - 1) / kTile + 1, sm_count, D);
+  if (code != FOCAL_E4M3 && code != FOCAL_INT8)
+    return set_error(FOCAL_ERR_UNSUPPORTED, "unsupported cache code (must be e4m3 or int8)");
+  const int per_seg = (max_seq_len - 1) / kTile + 1;
+  if ((long long)segs * per_seg > INT32_MAX / 2) return set_error(FOCAL_ERR_UNSUPPORTED, "segs * max_seq_len too large");
+  if (top < 0 || top > per_seg || total < 0 || total > segs * top)
+    return set_error(FOCAL_ERR_INVALID_VALUE, "top must be at most max_seq_len / 64, rounded up, and total at most segs * top");
+  const Plan plan = plan_for(segs, per_seg, sm_count, D);
   int ways = plan.ways, per = plan.per;
   if (plan.decide) {
     if (D == 128)

@@ -67,6 +67,8 @@ def test_plan_uses_the_gpu():
 
 def test_plan_refusals():
     L, out = _lib.lib(), (ctypes.c_int * 4)()
-    for args in ((0, 64, 128, 0, 148, 1, 1), (1, 0, 128, 0, 148, 1, 1), (1, 64, 128, 0, 0, 1, 1), (1, 64, 96, 0, 148, 1, 1)):
+    for args in ((0, 64, 128, 0, 148, 1, 1), (1, 0, 128, 0, 148, 1, 1), (1, 64, 128, 0, 0, 1, 1), (1, 64, 96, 0, 148, 1, 1),
+                 (1, 64, 128, 2, 148, 1, 1), (1 << 20, 1 << 20, 128, 0, 148, 1, 1), (1, 64, 128, 0, 148, 2, 2),
+                 (2, 64, 128, 0, 148, 3, 1), (1, 64, 128, 0, 148, -1, 1), (1, 64, 128, 0, 148, 0, -1)):
         assert L.focal_kv8_decode_plan(*args, out) != 0 and _lib.last_error()
     assert L.focal_kv8_decode_plan(1, 64, 128, 0, 148, 1, 1, None) == _lib.FOCAL_ERR_INVALID_VALUE
